@@ -479,6 +479,82 @@ int wj_bcast_weights(wj_comm* comm, void* blob_dev, int64_t bytes, int root, voi
 int wj_comm_count(wj_comm* comm, int* n_ranks_out);
 int wj_comm_destroy(wj_comm* comm);
 
+/* ---- 8-bit decoder step ------------------------------------------------------------------------
+ * The operators of a decoder layer whose products run on 8-bit integers and whose key / value cache holds 8-bit codes: the
+ * precision CTranslate2 offers the reference as compute_type="int8" (whisperjav/modules/faster_whisper_pro_asr.py:247-253 passes
+ * compute_type on; weights in int8, activations quantised per row as they are produced), plus the cache.
+ * A ROW of values x is held as int8 codes in [-127, 127] and one float32 scale: scale = max |x| / 127, code = x * (127 / max |x|)
+ * rounded to nearest, ties to even; x reads back as code * scale, off by at most scale / 2.  A row of zeros has scale 0.  A row that
+ * holds a NaN or an infinity has scale NaN and codes 0, so that it reads back as NaN and stays a single row's matter.
+ * Every call is asynchronous on `stream` and may be captured into a graph (no allocation, no copy, no memset inside); `stream` =
+ * WJ_STREAM_DEFAULT names the device's null stream (NULL is the context's own stream, as everywhere).  The caller's current device is
+ * left as it was.  Strides (ld*) are in elements and count from row to row; elements of a row are contiguous.  Outputs must not overlap
+ * inputs unless a parameter says so.  Calls with no rows do nothing.  wj_k_gemm_mx8 is the MX-fp8 relative. */
+#define WJ_STREAM_DEFAULT ((void*)(intptr_t)-1)
+
+/* r = x + delta; y = r / sqrt(mean(r^2) + eps) * w; codes, scale = y quantised per row.  x, residual: `dtype`; delta (NULL: none):
+ * `delta_dtype`; sums, norm and scale in float32 from the unrounded r.  residual (NULL: not stored) receives r rounded to `dtype` and may
+ * be x itself.  w float32 [cols].  1 <= cols <= 32768. */
+int wj_q8_rmsnorm(wj_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, int delta_dtype, const void* delta_dev, int64_t ldd,
+                  const float* w_dev, float eps, void* residual_dev, int64_t ldr, int8_t* codes_dev, int64_t ldc, float* scale_dev,
+                  int64_t rows, int cols, void* stream);
+/* codes, scale = rows of x quantised (swiglu_block 0), or rows of silu(gate) * up where x has 2 cols columns in alternating blocks of
+ * swiglu_block gate and swiglu_block up columns (swiglu_block divides cols; = cols: the two halves; 16: the Qwen engine's packed gate-up
+ * rows).  1 <= cols <= 32768. */
+int wj_q8_quantize(wj_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, int swiglu_block, int8_t* codes_dev, int64_t ldc,
+                   float* scale_dev, int64_t rows, int cols, void* stream);
+/* out [rows][cols] in `dtype` = code * scale, rounded once */
+int wj_q8_dequantize(wj_ctx* ctx, const int8_t* codes_dev, int64_t ldc, const float* scale_dev, int dtype, void* out_dev, int64_t ldo,
+                     int64_t rows, int cols, void* stream);
+/* out [m][n] in `dtype` = a_scale[i] * w_scale[j] * sum_k a[i][k] w[j][k] + bias[j] (bias float32 [n] or NULL).  The sum is exact
+ * (int32; codes may be -128 too, hence k <= 131071); the epilogue is float32, rounded once.  lda, ldw >= k.  Rows of codes that start at
+ * multiples of 16 bytes take the fast kernels (bytes between k and the next multiple of 16 are read and ignored, never written); any
+ * other base or stride is served, slower.  workspace_dev: at least wj_q8_gemm_workspace() bytes (may be 0 and NULL), used by this call
+ * alone until it is done on `stream`. */
+int64_t wj_q8_gemm_workspace(wj_ctx* ctx, int64_t m, int n, int k);
+int wj_q8_gemm(wj_ctx* ctx, const int8_t* a_dev, int64_t lda, const float* a_scale_dev, const int8_t* w_dev, int64_t ldw,
+               const float* w_scale_dev, const float* bias_dev, int dtype, void* out_dev, int64_t ldo, int64_t m, int n, int k,
+               void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* 8-bit key / value cache of one layer: codes [slots][heads][ctx][dim], scales [slots][heads][ctx], contiguous, codes 16-byte aligned.
+ * dim is 64 or 128.  A slot is a sequence's place; positions 0 .. ctx - 1. */
+typedef struct {
+  int8_t* k_dev;
+  float* k_scale_dev;
+  int8_t* v_dev;
+  float* v_scale_dev;
+  int32_t slots, heads, ctx, dim;
+} wj_kv8;
+/* The rows of a call: sequence b owns rows starts[b] .. starts[b + 1] - 1 of the row arrays and has lens[b] positions in the cache once
+ * they are written, so its row t (of n) sits at position lens[b] - n + t of slot slots[b].  All three arrays are int32 on the device
+ * (they may change between replays of a captured graph); starts has seqs + 1 entries and does not decrease.  rows = rows of the arrays:
+ * rows behind starts[seqs] are neither read nor written.  A sequence whose slot is outside 0 .. slots - 1 (a padded batch entry: -1)
+ * stores nothing, reads back as zeros and attends to nothing; so does, in writing and reading, a row whose position is outside
+ * 0 .. ctx - 1.  max_new, max_len: the most new rows and positions of any sequence -- hints that size the launch: a call whose arrays go
+ * past them is still right, only slower. */
+typedef struct {
+  const int32_t* slots_dev;
+  const int32_t* starts_dev;
+  const int32_t* lens_dev;
+  int32_t seqs, rows, max_new, max_len;
+} wj_kv8_batch;
+/* k, v rows [rows][heads][dim] in `dtype` -> codes and scales (a row of `dim` values per head) at their positions.  The slots of a call
+ * are distinct: of two sequences that write one position, which one's codes and which one's scale stay is not defined. */
+int wj_kv8_write(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int dtype, const void* k_dev, int64_t ldk, const void* v_dev,
+                 int64_t ldv, void* stream);
+/* the same positions read back as values, [rows][heads][dim] in `dtype` */
+int wj_kv8_read(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int dtype, void* k_dev, int64_t ldk, void* v_dev, int64_t ldv,
+                void* stream);
+/* out[row][h] = softmax_j(scale * q[row][h] . k_j) v_j over the cached positions j of the row's sequence, j <= the row's own position
+ * (causal != 0) or j < lens[b] (causal = 0: an encoder's states of another length, written once), the first ctx positions at most.
+ * q, out [rows][n_heads][dim] in `dtype`; query head h reads key / value head h / (n_heads / heads), n_heads <= 16 heads.  A row that
+ * sees no position (an empty cache, a causal row before position 0) is zeros.
+ * Positions behind are never let into a result, whatever the cache holds there.  Scores, softmax and sums are float32.
+ * workspace_dev: at least wj_kv8_attention_workspace() bytes (may be 0 and NULL), used by this call alone until it is done on `stream`. */
+int64_t wj_kv8_attention_workspace(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int n_heads);
+int wj_kv8_attention(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int dtype, const void* q_dev, int64_t ldq, void* out_dev,
+                     int64_t ldo, int n_heads, float scale, int causal, void* workspace_dev, int64_t workspace_bytes, void* stream);
+
 /* ---- kernel-level entry points (parity tests and micro-benchmarks only) ----------------- */
 /* C[M,N] = A[M,K] . W[N,K]^T + bias, plain row-major output in `dtype` (out_f32=0) or float32. */
 int wj_k_gemm(wj_ctx* ctx, int dtype, const void* a_dev, const void* w_dev, const float* bias_dev,

@@ -54,7 +54,7 @@ struct wj_ctx {
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
   int ensure_scratch(size_t bytes);
-  hipStream_t pick(void* s) const { return s ? reinterpret_cast<hipStream_t>(s) : stream; }
+  hipStream_t pick(void* s) const { return s == WJ_STREAM_DEFAULT ? nullptr : s ? reinterpret_cast<hipStream_t>(s) : stream; }
   // event-pair profiler (wj_profile_start/stop): per-tag kernel time measured with HIP events on the
   // stream the kernels are launched on
   struct wj_profiler* prof = nullptr;

@@ -1,0 +1,66 @@
+// q8.hpp -- what the 8-bit operators (q8.hip, kv8.hip) share: element access by run-time type, row quantisation, host-side checks.
+#pragma once
+
+#include <math.h>
+
+#include "kernels.hpp"
+
+namespace wj {
+
+// the calling thread's device is put back on every way out of an entry point
+struct DeviceScope {
+  int prev = -1;
+  hipError_t enter(int device) {
+    hipError_t e = hipGetDevice(&prev);
+    if (e != hipSuccess) { prev = -1; return e; }
+    if (prev == device) { prev = -1; return hipSuccess; }
+    return hipSetDevice(device);
+  }
+  ~DeviceScope() { if (prev >= 0) (void)hipSetDevice(prev); }
+};
+
+inline bool known_dtype(int dtype) { return dtype == WJ_F32 || is16(dtype); }
+inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// one element of a row whose type is known at run time only (wave-uniform)
+__device__ __forceinline__ float ld_any(const void* p, int dtype, int64_t i) {
+  if (dtype == WJ_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == WJ_F16) return h2f(reinterpret_cast<const f16_t*>(p)[i]);
+  return bf2f(reinterpret_cast<const bf16_t*>(p)[i]);
+}
+
+// bfloat16 of any float, NaN included (f2bf's carry can turn a NaN's payload into an infinity)
+__device__ __forceinline__ bf16_t f2bf_any(float v) { return v != v ? (bf16_t)0x7fc0u : f2bf(v); }
+template <typename T> __device__ __forceinline__ T to_T(float v);
+template <> __device__ __forceinline__ float to_T<float>(float v) { return v; }
+template <> __device__ __forceinline__ f16_t to_T<f16_t>(float v) { return f2h(v); }
+template <> __device__ __forceinline__ bf16_t to_T<bf16_t>(float v) { return f2bf_any(v); }
+
+__device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
+  if (dtype == WJ_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == WJ_F16) reinterpret_cast<f16_t*>(p)[i] = f2h(v);
+  else reinterpret_cast<bf16_t*>(p)[i] = f2bf_any(v);
+}
+
+// magnitude that carries "not finite" through a maximum: fmaxf alone drops a NaN
+__device__ __forceinline__ float mag(float v) { const float a = fabsf(v); return a < INFINITY ? a : INFINITY; }
+
+// The quantiser of a row with maximum magnitude `amax` (INFINITY: the row holds a NaN or an infinity): code = rint(v * (127 / amax)),
+// scale = amax / 127.  Below 1e-30 the quotient would run out of range, so values and maximum are lifted by 2^80 first (exact).
+struct RowQuant {
+  float scale, lift, inv;
+  bool live;
+  __device__ __forceinline__ explicit RowQuant(float amax) {
+    live = amax > 0.f && amax < INFINITY;
+    lift = amax < 1e-30f ? 1.2089258196146292e24f : 1.f;
+    inv = live ? 127.f / (amax * lift) : 0.f;
+    scale = amax < INFINITY ? amax / 127.f : __uint_as_float(0x7fc00000u);
+  }
+  __device__ __forceinline__ int code(float v) const { return live ? (int)rintf(v * lift * inv) : 0; }
+};
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+  return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) | ((uint32_t)d << 24);
+}
+
+}  // namespace wj

@@ -121,6 +121,15 @@ _SIGNATURES = {
     "wj_bcast_weights": (_I, [_P, _P, _I64, _I, _P]),
     "wj_comm_count": (_I, [_P, C.POINTER(_I)]),
     "wj_comm_destroy": (_I, [_P]),
+    "wj_q8_rmsnorm": (_I, [_P, _I, _P, _I64, _I, _P, _I64, _P, _F, _P, _I64, _P, _I64, _P, _I64, _I, _P]),
+    "wj_q8_quantize": (_I, [_P, _I, _P, _I64, _I, _P, _I64, _P, _I64, _I, _P]),
+    "wj_q8_dequantize": (_I, [_P, _P, _I64, _P, _I, _P, _I64, _I64, _I, _P]),
+    "wj_q8_gemm_workspace": (_I64, [_P, _I64, _I, _I]),
+    "wj_q8_gemm": (_I, [_P, _P, _I64, _P, _P, _I64, _P, _P, _I, _P, _I64, _I64, _I, _I, _P, _I64, _P]),
+    "wj_kv8_write": (_I, [_P, _P, _P, _I, _P, _I64, _P, _I64, _P]),
+    "wj_kv8_read": (_I, [_P, _P, _P, _I, _P, _I64, _P, _I64, _P]),
+    "wj_kv8_attention_workspace": (_I64, [_P, _P, _P, _I]),
+    "wj_kv8_attention": (_I, [_P, _P, _P, _I, _P, _I64, _P, _I64, _I, _F, _I, _P, _I64, _P]),
     "wj_k_gemm": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "wj_k_gemm_split": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "wj_k_gemm_timed": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, C.POINTER(_F)]),
