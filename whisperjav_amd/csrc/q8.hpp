@@ -45,18 +45,24 @@ __device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
 // magnitude that carries "not finite" through a maximum: fmaxf alone drops a NaN
 __device__ __forceinline__ float mag(float v) { const float a = fabsf(v); return a < INFINITY ? a : INFINITY; }
 
-// The quantiser of a row with maximum magnitude `amax` (INFINITY: the row holds a NaN or an infinity): code = rint(v * (127 / amax)),
-// scale = amax / 127.  Below 1e-30 the quotient would run out of range, so values and maximum are lifted by 2^80 first (exact).
+// The quantiser of a row with maximum magnitude `amax` (INFINITY: the row holds a NaN or an infinity): scale = amax / 127, code =
+// rint(v / scale).  The quotient is the rounded one (a reciprocal, then one correction): v = amax / 2 is the tie 63.5 and common among
+// 16-bit values, so a product with 127 / amax that misses it moves a code of every such row.  Below 1e-30 values and maximum are lifted
+// by 2^80 first (exact), where scale itself would lose its last bits.
 struct RowQuant {
-  float scale, lift, inv;
+  float scale, lift, step, inv;
   bool live;
   __device__ __forceinline__ explicit RowQuant(float amax) {
     live = amax > 0.f && amax < INFINITY;
     lift = amax < 1e-30f ? 1.2089258196146292e24f : 1.f;
-    inv = live ? 127.f / (amax * lift) : 0.f;
+    step = live ? amax * lift / 127.f : 1.f;
+    inv = 1.f / step;
     scale = amax < INFINITY ? amax / 127.f : __uint_as_float(0x7fc00000u);
   }
-  __device__ __forceinline__ int code(float v) const { return live ? (int)rintf(v * lift * inv) : 0; }
+  __device__ __forceinline__ int code(float v) const {
+    const float x = v * lift, t = x * inv;
+    return live ? (int)rintf(fmaf(fmaf(-t, step, x), inv, t)) : 0;
+  }
 };
 
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
