@@ -225,7 +225,10 @@ __global__ __launch_bounds__(256) void q8_dequantize_kernel(const int8_t* __rest
 }
 
 // --------------------------------------------------------------------------------------------
-// int8 product
+// int8 product.  v_mfma_i32_16x16x64_i8: a lane's operand is 16 consecutive codes of one row, so an int8 tile lies in LDS exactly as a
+// 16-bit tile of half the columns would, and twice the products come out of the same bytes.  The weights go first, which leaves a lane with
+// 4 consecutive output columns of one row.  Codes past k inside a row's last 16 bytes may be anything: they are cleared on the activations'
+// side, which is enough.  int32 sums are exact, so the kernels agree bit for bit whatever their order.
 // --------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 
@@ -233,14 +236,415 @@ struct GemmQ8Args {
   const int8_t* a; int64_t lda; const float* sa;
   const int8_t* w; int64_t ldw; const float* sw;
   const float* bias;
-  void* out; int64_t ldo; int dtype;
+  void* out; int64_t ldo;
   int64_t m; int n, k;
+  int32_t* slab; int ksplit;           // ksplit > 1: raw sums [ksplit][m][n] instead of out
 };
 
 __device__ __forceinline__ i32x4_t mfma_i8(i32x4_t a, i32x4_t b, i32x4_t c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
+// the bytes of a 16-byte piece that lie before `valid` (<= 0: none, >= 16: all)
+__device__ __forceinline__ i32x4_t piece_mask(int valid) {
+  i32x4_t m;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const int b = min(4, max(0, valid - 4 * d));
+    m[d] = b == 4 ? -1 : (int)((1u << (8 * b)) - 1u);
+  }
+  return m;
+}
+
+// Barrier without the fence of __syncthreads(), which would wait for every LDS-DMA request in flight: the kernels order their LDS
+// traffic themselves (a counted s_waitcnt vmcnt by the waves that issued the DMA, the barrier, then the reads; s_waitcnt lgkmcnt(0) by
+// the readers before the barrier that hands a buffer back).
+__device__ __forceinline__ void q8_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void dma16(const int8_t* src, int8_t* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+__device__ __forceinline__ void ld4_to(const float* p, int n, int limit, float v[4]) {       // p[n .. n + 3], clamped below `limit`
+  if (n + 4 <= limit) __builtin_memcpy(v, p + n, 16);
+  else
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = p[min(n + e, limit - 1)];
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack_any(float lo, float hi) {
+  return (uint32_t)__builtin_bit_cast(uint16_t, to_T<T>(lo)) | ((uint32_t)__builtin_bit_cast(uint16_t, to_T<T>(hi)) << 16);
+}
+
+// out = acc * (sa * sw) + bias of RI x 4 fragments of 16 x 16, wave origin (mw, nw).  16-bit types: lanes 16 apart trade halves of
+// neighbouring fragments (v_permlane16_swap), so that a lane stores 8 consecutive columns at once.
+template <typename T, int RI>
+__device__ __forceinline__ void q8_epilogue(const GemmQ8Args& g, int64_t mw, int nw, int lane, i32x4_t (&acc)[RI][4]) {
+  const int li = lane & 15, q = lane >> 4;
+  float sw[4][4], bias[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = nw + j * 16 + q * 4;
+    ld4_to(g.sw, n, g.n, sw[j]);
+    if (g.bias) ld4_to(g.bias, n, g.n, bias[j]);
+    else
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[j][e] = 0.f;
+  }
+  float sa[RI];
+#pragma unroll
+  for (int i = 0; i < RI; ++i) sa[i] = g.sa[min(mw + i * 16 + li, g.m - 1)];
+#pragma unroll
+  for (int i = 0; i < RI; ++i) {
+    const int64_t m = mw + i * 16 + li;
+    T* row = reinterpret_cast<T*>(g.out) + min(m, g.m - 1) * g.ldo;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = nw + j * 16 + q * 4;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * (sa[i] * sw[j][e]) + bias[j][e];
+        if (m < g.m) {
+          if (n + 4 <= g.n) __builtin_memcpy(row + n, v, 16);
+          else
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+              if (n + e < g.n) row[n + e] = v[e];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int jp = 0; jp < 4; jp += 2) {
+        float va[4], vb[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          va[e] = (float)acc[i][jp][e] * (sa[i] * sw[jp][e]) + bias[jp][e];
+          vb[e] = (float)acc[i][jp + 1][e] * (sa[i] * sw[jp + 1][e]) + bias[jp + 1][e];
+        }
+        const uint32_t a0 = pack_any<T>(va[0], va[1]), a1 = pack_any<T>(va[2], va[3]);
+        const uint32_t b0 = pack_any<T>(vb[0], vb[1]), b1 = pack_any<T>(vb[2], vb[3]);
+        const auto s0 = __builtin_amdgcn_permlane16_swap(a0, b0, false, false);
+        const auto s1 = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
+        const uint32_t w[4] = {(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
+        const int n8 = nw + (jp + (q & 1)) * 16 + (q >> 1) * 8;
+        if (m < g.m) {
+          if (n8 + 8 <= g.n) __builtin_memcpy(row + n8, w, 16);
+          else
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+              if (n8 + e < g.n) reinterpret_cast<uint16_t*>(row)[n8 + e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+        }
+      }
+    }
+  }
+}
+
+// Tile order: workgroups go to the 8 XCDs in turn, so each XCD takes a contiguous run of tiles, in groups of 8 row panels walked column by
+// column: an XCD's L2 sees few panels of either operand at a time.
+__device__ __forceinline__ void tile_of(int lin, int nx, int ny, int* tx, int* ty) {
+  const int total = nx * ny, q8 = total >> 3, r8 = total & 7, xcd = lin & 7;
+  const int tile = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (lin >> 3);
+  const int per_group = 8 * nx, group = tile / per_group, first = group * 8, rows = min(8, ny - first), in = tile - group * per_group;
+  *ty = first + in % rows;
+  *tx = in / rows;
+}
+
+// 256 x 256 tile, 8 waves (2 x 4, 128 x 64 each), k in pairs of 64 + 64 codes (128-byte row segments), two 64 KiB buffers.  The two waves of
+// every SIMD run one barrier apart: one group reads its fragments (and requests the next pair) while the other runs 32 products on
+// fragments in registers.  Barrier sequence after the prologue barrier P, every wave in every barrier:
+//   group 0:        MEM(0) B0 MFMA(0) B1 MEM(1) B2 MFMA(1) B3 ...      group 1:  B0 MEM(0) B1 MFMA(0) B2 MEM(1) B3 ...
+//   MEM(2p) reads half 0 of pair p and requests pair p + 1 into the other buffer; MEM(2p + 1) reads half 1 and waits for the requests.
+// WAR: the other buffer held pair p - 1, read last in group 1's MEM(2p - 1), retired before B(4p - 1); MEM(2p) starts after it.
+// RAW: both groups have waited for pair p + 1 by B(4p + 3); it is first read after that.
+// 128-byte LDS rows, 16-byte piece c of row r in place c ^ (r & 7).
+template <typename T>
+__global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, int nx, int ny) {
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [buffer][A | W][256][128]
+  constexpr int STAGE = 2 * 256 * 128;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  int tx, ty;
+  tile_of(blockIdx.x, nx, ny, &tx, &ty);
+  const int64_t m0 = (int64_t)ty * 256;
+  const int n0 = tx * 256;
+  const int8_t* ga[4];
+  const int8_t* gw[4];
+  const int c = (lane & 7) ^ ((lane >> 3) & 7);                    // rows of a request start at multiples of 8: row & 7 = lane >> 3
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int row = (wave * 4 + q) * 8 + (lane >> 3);
+    ga[q] = g.a + min(m0 + row, g.m - 1) * g.lda + c * 16;
+    gw[q] = g.w + (int64_t)min(n0 + row, g.n - 1) * g.ldw + c * 16;
+  }
+  const int np = (g.k + 127) / 128;
+  // pieces that lie wholly past k are fetched from the row's start instead (in bounds; cleared below like every code past k)
+  auto issue = [&](int p, int buf) __attribute__((always_inline)) {
+    const int back = p == np - 1 && p * 128 + c * 16 >= g.k ? p * 128 + c * 16 : 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      dma16(ga[q] - back, &lds[buf * STAGE + (wave * 4 + q) * 1024]);
+      dma16(gw[q] - back, &lds[buf * STAGE + 256 * 128 + (wave * 4 + q) * 1024]);
+      ga[q] += 128;
+      gw[q] += 128;
+    }
+  };
+  i32x4_t acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+  const int off0 = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const int off1 = (lane & 15) * 128 + (((4 + (lane >> 4)) ^ (lane & 7)) << 4);
+  const int a_base = wm * 128 * 128, w_base = 256 * 128 + wn * 64 * 128;
+
+  issue(0, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  q8_barrier();                 // P
+  if (wm == 1) q8_barrier();    // B0
+  i32x4_t af[8], wf[4];
+#define WJ_Q8_READ(buf, off)                                                                                                    \
+  {                                                                                                                             \
+    const int8_t* ls = &lds[(buf) * STAGE];                                                                                     \
+    _Pragma("unroll") for (int j = 0; j < 4; ++j) wf[j] = *reinterpret_cast<const i32x4_t*>(&ls[w_base + j * 2048 + (off)]);    \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) af[i] = *reinterpret_cast<const i32x4_t*>(&ls[a_base + i * 2048 + (off)]);    \
+  }
+#define WJ_Q8_CLEAR(h)                                                                       \
+  if (p == np - 1 && (g.k & 127)) {                                                          \
+    const i32x4_t mask = piece_mask(g.k - (p * 128 + (h) * 64 + (lane >> 4) * 16));          \
+    _Pragma("unroll") for (int i = 0; i < 8; ++i) af[i] &= mask;                             \
+  }
+#define WJ_Q8_MFMA()                                                                         \
+  __builtin_amdgcn_s_setprio(1);                                                             \
+  _Pragma("unroll") for (int i = 0; i < 8; ++i)                                              \
+    _Pragma("unroll") for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(wf[j], af[i], acc[i][j]); \
+  __builtin_amdgcn_s_setprio(0);
+  for (int p = 0; p < np; ++p) {
+    const int b = p & 1;
+    WJ_Q8_READ(b, off0)
+    if (p + 1 < np) issue(p + 1, b ^ 1);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    WJ_Q8_CLEAR(0)
+    q8_barrier();
+    WJ_Q8_MFMA()
+    q8_barrier();
+    WJ_Q8_READ(b, off1)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    WJ_Q8_CLEAR(1)
+    q8_barrier();
+    WJ_Q8_MFMA()
+    q8_barrier();
+  }
+  if (wm == 0) q8_barrier();    // every wave has taken part in the same number of barriers
+#undef WJ_Q8_READ
+#undef WJ_Q8_CLEAR
+#undef WJ_Q8_MFMA
+  q8_epilogue<T, 8>(g, m0 + wm * 128, n0 + wn * 64, lane, acc);
+}
+
+// BM x 128 tile, 4 waves (2 x 2, BM / 2 x 64 each), k steps of 128 codes, a ring of NS buffers with NS - 1 steps requested ahead.  For
+// calls with too few 256-tiles to fill the chip; ksplit > 1: slices of k on the grid's second axis write raw sums, joined by
+// q8_gemm_join_kernel.
+template <typename T, int BM, int NS>
+__global__ __launch_bounds__(256) void q8_gemm_tile_kernel(const GemmQ8Args g, int nx, int ny) {
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [stage][A: BM | W: 128][128]
+  constexpr int STAGE = (BM + 128) * 128, RI = BM / 32, QA = BM / 32;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  int tx, ty;
+  tile_of(blockIdx.x, nx, ny, &tx, &ty);
+  const int64_t m0 = (int64_t)ty * BM;
+  const int n0 = tx * 128;
+  const int steps = (g.k + 127) / 128;
+  const int s_begin = (int)((int64_t)steps * blockIdx.y / g.ksplit), s_end = (int)((int64_t)steps * (blockIdx.y + 1) / g.ksplit);
+  const int nk = s_end - s_begin;
+  const int c = (lane & 7) ^ ((lane >> 3) & 7);
+  const int8_t* ga[QA];
+  const int8_t* gw[4];
+#pragma unroll
+  for (int q = 0; q < QA; ++q) ga[q] = g.a + min(m0 + (wave * QA + q) * 8 + (lane >> 3), g.m - 1) * g.lda + c * 16 + (int64_t)s_begin * 128;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) gw[q] = g.w + (int64_t)min(n0 + (wave * 4 + q) * 8 + (lane >> 3), g.n - 1) * g.ldw + c * 16 + (int64_t)s_begin * 128;
+  auto issue = [&](int s, int buf) __attribute__((always_inline)) {
+    const int back = s == steps - 1 && s * 128 + c * 16 >= g.k ? s * 128 + c * 16 : 0;
+#pragma unroll
+    for (int q = 0; q < QA; ++q) { dma16(ga[q] - back, &lds[buf * STAGE + (wave * QA + q) * 1024]); ga[q] += 128; }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { dma16(gw[q] - back, &lds[buf * STAGE + BM * 128 + (wave * 4 + q) * 1024]); gw[q] += 128; }
+  };
+  i32x4_t acc[RI][4];
+#pragma unroll
+  for (int i = 0; i < RI; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+  for (int st = 0; st < NS - 1; ++st)
+    if (st < nk) issue(s_begin + st, st);
+  int buf = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    constexpr int PER = QA + 4;                        // requests of a step
+    const int younger = min(NS - 2, nk - 1 - kt);      // steps requested after kt that may stay in flight
+    if (younger >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
+    else if (younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // step kt is visible to all; the buffer of step kt - 1 is free (its reads were retired before this barrier)
+    q8_barrier();
+    if (kt + NS - 1 < nk) issue(s_begin + kt + NS - 1, buf == 0 ? NS - 1 : buf - 1);
+    const int8_t* la = &lds[buf * STAGE];
+    const int8_t* lw = la + BM * 128;
+    i32x4_t af[2][RI], wf[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int off = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
+#pragma unroll
+      for (int i = 0; i < RI; ++i) af[h][i] = *reinterpret_cast<const i32x4_t*>(&la[(wm * (BM / 2) + i * 16) * 128 + off]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wf[h][j] = *reinterpret_cast<const i32x4_t*>(&lw[(wn * 64 + j * 16) * 128 + off]);
+    }
+    if (s_begin + kt == steps - 1 && (g.k & 127)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const i32x4_t mask = piece_mask(g.k - ((s_begin + kt) * 128 + h * 64 + (lane >> 4) * 16));
+#pragma unroll
+        for (int i = 0; i < RI; ++i) af[h][i] &= mask;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < RI; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(wf[h][j], af[h][i], acc[i][j]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    buf = buf == NS - 1 ? 0 : buf + 1;
+  }
+  const int64_t mw = m0 + wm * (BM / 2);
+  const int nw = n0 + wn * 64;
+  if (g.ksplit == 1) {
+    q8_epilogue<T, RI>(g, mw, nw, lane, acc);
+    return;
+  }
+  int32_t* slab = g.slab + (int64_t)blockIdx.y * g.m * g.n;
+#pragma unroll
+  for (int i = 0; i < RI; ++i) {
+    const int64_t m = mw + i * 16 + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = nw + j * 16 + (lane >> 4) * 4;
+      if (m < g.m) {
+        if (n + 4 <= g.n) __builtin_memcpy(slab + m * g.n + n, &acc[i][j], 16);
+        else
+#pragma unroll
+          for (int e = 0; e < 3; ++e)
+            if (n + e < g.n) slab[m * g.n + n + e] = acc[i][j][e];
+      }
+    }
+  }
+}
+
+// out = epilogue of the slices' sums, 4 columns per lane
+template <typename T>
+__global__ __launch_bounds__(256) void q8_gemm_join_kernel(const GemmQ8Args g) {
+  const int groups = (g.n + 3) >> 2;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= g.m * groups) return;
+  const int64_t m = i / groups;
+  const int n = (int)(i - m * groups) * 4;
+  int sum[4] = {0, 0, 0, 0};
+  float sw[4], bias[4] = {0.f, 0.f, 0.f, 0.f};
+  ld4_to(g.sw, n, g.n, sw);
+  if (g.bias) ld4_to(g.bias, n, g.n, bias);
+  const float sa = g.sa[m];
+  const bool whole = n + 4 <= g.n;
+  for (int s = 0; s < g.ksplit; ++s) {
+    const int32_t* p = g.slab + ((int64_t)s * g.m + m) * g.n + n;
+    int v[4] = {0, 0, 0, 0};
+    if (whole) __builtin_memcpy(v, p, 16);
+    else
+      for (int e = 0; n + e < g.n; ++e) v[e] = p[e];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += v[e];
+  }
+  T t[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) t[e] = to_T<T>((float)sum[e] * (sa * sw[e]) + bias[e]);
+  T* o = reinterpret_cast<T*>(g.out) + m * g.ldo + n;
+  if (whole) __builtin_memcpy(o, t, sizeof(t));
+  else
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (n + e < g.n) o[e] = t[e];
+}
+
+// Few rows (at most 16 MT): bound by the weights' bytes.  A workgroup owns 16 output columns, its 8 waves split k, the weights go straight
+// from memory into the operands (every byte once), the 8 partial tiles meet in LDS.
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void q8_gemm_rows_kernel(const GemmQ8Args g) {
+  __shared__ __attribute__((aligned(16))) int red[8 * MT * 256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  constexpr int UNR = MT == 1 ? 4 : 2;
+  const int steps = (g.k + 63) / 64, per = (steps + 7) / 8;
+  const int s_begin = wave * per, s_end = min(steps, s_begin + per);
+  const int8_t* wr = g.w + (int64_t)min(n0 + li, g.n - 1) * g.ldw;
+  i32x4_t acc[MT];
+  const int8_t* ar[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    acc[t] = i32x4_t{0, 0, 0, 0};
+    ar[t] = g.a + min((int64_t)t * 16 + li, g.m - 1) * g.lda;
+  }
+  for (int s0 = s_begin; s0 < s_end; s0 += UNR) {
+    i32x4_t wv[UNR], av[UNR][MT];
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) {
+      const int k = (s0 + u) * 64 + q * 16;
+      const bool in = s0 + u < s_end && k < g.k;
+      const int kc = in ? k : 0;
+      wv[u] = *reinterpret_cast<const i32x4_t*>(wr + kc);
+      const i32x4_t mask = piece_mask(in ? g.k - k : 0);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) av[u][t] = *reinterpret_cast<const i32x4_t*>(ar[t] + kc) & mask;
+    }
+#pragma unroll
+    for (int u = 0; u < UNR; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[t] = mfma_i8(wv[u], av[u][t], acc[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) *reinterpret_cast<i32x4_t*>(&red[(wave * MT * 16 + t * 16 + li) * 16 + q * 4]) = acc[t];
+  __syncthreads();
+  for (int o = tid; o < MT * 64; o += 512) {
+    const int64_t m = o >> 2;
+    const int n = n0 + (o & 3) * 4;
+    if (m >= g.m || n >= g.n) continue;
+    i32x4_t sum = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += *reinterpret_cast<const i32x4_t*>(&red[(w * MT * 16 + (int)m) * 16 + (o & 3) * 4]);
+    float sw[4], bias[4] = {0.f, 0.f, 0.f, 0.f};
+    ld4_to(g.sw, n, g.n, sw);
+    if (g.bias) ld4_to(g.bias, n, g.n, bias);
+    const float sa = g.sa[m];
+    T* row = reinterpret_cast<T*>(g.out) + m * g.ldo + n;
+    T t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = to_T<T>((float)sum[e] * (sa * sw[e]) + bias[e]);
+    if (n + 4 <= g.n) __builtin_memcpy(row, t, sizeof(t));
+    else
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (n + e < g.n) row[e] = t[e];
+  }
+}
+
 // Any base, stride and size: 64 x 64 tile, k step 64, operands gathered byte by byte into LDS, 4 waves of 16 rows x 64 columns.
-__global__ __launch_bounds__(256) void q8_gemm_any_kernel(const GemmQ8Args g) {
+__global__ __launch_bounds__(256) void q8_gemm_any_kernel(const GemmQ8Args g, int dtype) {
   __shared__ __attribute__((aligned(16))) int8_t la[64 * 80], lw[64 * 80];      // rows 80 bytes apart: 16-byte reads, few bank conflicts
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t m0 = (int64_t)blockIdx.y * 64;
@@ -272,7 +676,7 @@ __global__ __launch_bounds__(256) void q8_gemm_any_kernel(const GemmQ8Args g) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int n = n0 + j * 16 + (lane >> 4) * 4 + e;
-      if (n < g.n) st_any(g.out, g.dtype, m * g.ldo + n, (float)acc[j][e] * (sa * g.sw[n]) + (g.bias ? g.bias[n] : 0.f));
+      if (n < g.n) st_any(g.out, dtype, m * g.ldo + n, (float)acc[j][e] * (sa * g.sw[n]) + (g.bias ? g.bias[n] : 0.f));
     }
 }
 
@@ -310,6 +714,72 @@ int launch_rows(wj_ctx* ctx, int dtype, int delta_dtype, const RowArgs& a, void*
   if (dtype == WJ_F32) return pick_delta<MODE, float>(a, delta_dtype, s);
   if (dtype == WJ_F16) return pick_delta<MODE, f16_t>(a, delta_dtype, s);
   return pick_delta<MODE, bf16_t>(a, delta_dtype, s);
+}
+
+// Which kernel a product takes, from its size alone (the workspace follows from it)
+enum GemmKind { GEMM_ROWS, GEMM_BIG, GEMM_TILE128, GEMM_TILE64 };
+struct GemmPlan { GemmKind kind; int ksplit; };
+GemmPlan plan_gemm(int64_t m, int n, int k) {
+  if (m <= 64) return {GEMM_ROWS, 1};
+  const int64_t t256 = ((m + 255) / 256) * ((n + 255) / 256), t128 = ((m + 127) / 128) * ((n + 127) / 128), t64 = ((m + 63) / 64) * ((n + 127) / 128);
+  if (t256 >= 192) return {GEMM_BIG, 1};
+  if (t128 >= 256) return {GEMM_TILE128, 1};
+  const int steps = (k + 127) / 128;
+  int ks = 1;
+  while (ks < 8 && t64 * ks * 2 <= 512 && steps >= 4 * ks * 2) ks *= 2;
+  return {GEMM_TILE64, ks};
+}
+
+template <typename K>
+int allow_lds(K kernel, AttrOnce& once, int bytes) {
+  if (once.need()) {
+    WJ_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    once.done();
+  }
+  return WJ_OK;
+}
+
+template <typename T, int BM, int NS>
+int start_tile(const GemmQ8Args& g, hipStream_t s) {
+  static AttrOnce once;
+  constexpr int lds = NS * (BM + 128) * 128;
+  if (int rc = allow_lds(q8_gemm_tile_kernel<T, BM, NS>, once, lds)) return rc;
+  const int nx = (g.n + 127) / 128, ny = (int)((g.m + BM - 1) / BM);
+  hipLaunchKernelGGL((q8_gemm_tile_kernel<T, BM, NS>), dim3((unsigned)nx * ny, g.ksplit), dim3(256), lds, s, g, nx, ny);
+  WJ_LAUNCH_CHECK();
+  if (g.ksplit > 1) {
+    const int64_t threads = g.m * ((g.n + 3) / 4);
+    hipLaunchKernelGGL(q8_gemm_join_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g);
+    WJ_LAUNCH_CHECK();
+  }
+  return WJ_OK;
+}
+
+template <typename T>
+int launch_gemm_q8(GemmQ8Args g, hipStream_t s) {
+  const GemmPlan p = plan_gemm(g.m, g.n, g.k);
+  g.ksplit = p.ksplit;
+  switch (p.kind) {
+    case GEMM_ROWS: {
+      const dim3 grid((unsigned)((g.n + 15) / 16));
+      if (g.m <= 16) hipLaunchKernelGGL((q8_gemm_rows_kernel<T, 1>), grid, dim3(512), 0, s, g);
+      else if (g.m <= 32) hipLaunchKernelGGL((q8_gemm_rows_kernel<T, 2>), grid, dim3(512), 0, s, g);
+      else hipLaunchKernelGGL((q8_gemm_rows_kernel<T, 4>), grid, dim3(512), 0, s, g);
+      WJ_LAUNCH_CHECK();
+      return WJ_OK;
+    }
+    case GEMM_BIG: {
+      static AttrOnce once;
+      constexpr int lds = 2 * 2 * 256 * 128;
+      if (int rc = allow_lds(q8_gemm_big_kernel<T>, once, lds)) return rc;
+      const int nx = (g.n + 255) / 256, ny = (int)((g.m + 255) / 256);
+      hipLaunchKernelGGL(q8_gemm_big_kernel<T>, dim3((unsigned)nx * ny), dim3(512), lds, s, g, nx, ny);
+      WJ_LAUNCH_CHECK();
+      return WJ_OK;
+    }
+    case GEMM_TILE128: return start_tile<T, 128, 3>(g, s);
+    default: return start_tile<T, 64, 3>(g, s);
+  }
 }
 
 }  // namespace
@@ -364,8 +834,10 @@ int wj_q8_dequantize(wj_ctx* ctx, const int8_t* codes_dev, int64_t ldc, const fl
 }
 
 int64_t wj_q8_gemm_workspace(wj_ctx* ctx, int64_t m, int n, int k) {
-  (void)ctx; (void)m; (void)n; (void)k;
-  return 0;
+  (void)ctx;
+  if (m <= 0 || n <= 0 || k < 0) return 0;
+  const GemmPlan p = plan_gemm(m, n, k);
+  return p.ksplit > 1 ? (int64_t)p.ksplit * m * n * 4 : 0;
 }
 
 int wj_q8_gemm(wj_ctx* ctx, const int8_t* a_dev, int64_t lda, const float* a_scale_dev, const int8_t* w_dev, int64_t ldw,
@@ -382,10 +854,19 @@ int wj_q8_gemm(wj_ctx* ctx, const int8_t* a_dev, int64_t lda, const float* a_sca
              (long long)wj_q8_gemm_workspace(ctx, m, n, k));
   DeviceScope dev;
   WJ_HIP(dev.enter(ctx->device));
-  const GemmQ8Args g{a_dev, lda, a_scale_dev, w_dev, ldw, w_scale_dev, bias_dev, out_dev, ldo, dtype, m, n, k};
-  hipLaunchKernelGGL(q8_gemm_any_kernel, dim3((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64)), dim3(256), 0, ctx->pick(stream), g);
+  hipStream_t s = ctx->pick(stream);
+  const GemmQ8Args g{a_dev, lda, a_scale_dev, w_dev, ldw, w_scale_dev, bias_dev, out_dev, ldo, m, n, k, reinterpret_cast<int32_t*>(workspace_dev), 1};
+  // the fast kernels fetch rows in 16-byte pieces
+  const bool pieces = aligned_to(a_dev, 16) && aligned_to(w_dev, 16) && (m == 1 || lda % 16 == 0) && (n == 1 || ldw % 16 == 0);
+  if (pieces && k > 0) {
+    WJ_REQUIRE(workspace_dev || wj_q8_gemm_workspace(ctx, m, n, k) == 0, "wj_q8_gemm: NULL workspace");
+    WJ_REQUIRE(aligned_to(workspace_dev, 16), "wj_q8_gemm: the workspace is not 16-byte aligned");
+    if (dtype == WJ_F32) return launch_gemm_q8<float>(g, s);
+    if (dtype == WJ_F16) return launch_gemm_q8<f16_t>(g, s);
+    return launch_gemm_q8<bf16_t>(g, s);
+  }
+  hipLaunchKernelGGL(q8_gemm_any_kernel, dim3((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64)), dim3(256), 0, s, g, dtype);
   WJ_LAUNCH_CHECK();
-  (void)workspace_dev;
   return WJ_OK;
 }
 
