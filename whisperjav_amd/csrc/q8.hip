@@ -447,130 +447,129 @@ __global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, in
   q8_epilogue<T, 8>(g, m0 + wm * 128, n0 + wn * 64, lane, acc);
 }
 
-// BM x 128 tile, 4 waves (2 x 2, BM / 2 x 64 each), k steps of 128 codes, a ring of NS buffers with NS - 1 steps requested ahead.  For
-// calls with too few 256-tiles to fill the chip; ksplit > 1: slices of k on the grid's second axis write raw sums, joined by
-// q8_gemm_join_kernel.
-template <typename T, int BM, int NS>
-__global__ __launch_bounds__(256) void q8_gemm_tile_kernel(const GemmQ8Args g, int nx, int ny) {
-  extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [stage][A: BM | W: 128][128]
-  constexpr int STAGE = (BM + 128) * 128, RI = BM / 32, QA = BM / 32;
+// 64 x 128 tile, k steps of 128 codes, a ring of NS buffers with NS - 1 steps requested ahead.  Eight waves: (2 x 2, 32 x 64 each) twice,
+// each four taking one half of every step's codes, so that the two waves of a SIMD overlap one's LDS reads with the other's products; the
+// two halves' sums meet in LDS at the end, each four finishing 16 of every 32 rows.  For calls with too few 256-tiles to fill the chip;
+// ksplit > 1: slices of k on the grid's second axis write raw sums, joined by q8_gemm_join_kernel.
+template <typename T, int NS>
+__global__ __launch_bounds__(512) void q8_gemm_tile_kernel(const GemmQ8Args g, int nx, int ny) {
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [stage][A: 64 | W: 128][128]
+  constexpr int STAGE = (64 + 128) * 128;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int half = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
   int tx, ty;
   tile_of(blockIdx.x, nx, ny, &tx, &ty);
-  const int64_t m0 = (int64_t)ty * BM;
+  const int64_t m0 = (int64_t)ty * 64;
   const int n0 = tx * 128;
   const int steps = (g.k + 127) / 128;
   const int s_begin = (int)((int64_t)steps * blockIdx.y / g.ksplit), s_end = (int)((int64_t)steps * (blockIdx.y + 1) / g.ksplit);
   const int nk = s_end - s_begin;
   const int c = (lane & 7) ^ ((lane >> 3) & 7);
-  const int8_t* ga[QA];
-  const int8_t* gw[4];
-#pragma unroll
-  for (int q = 0; q < QA; ++q) ga[q] = g.a + min(m0 + (wave * QA + q) * 8 + (lane >> 3), g.m - 1) * g.lda + c * 16 + (int64_t)s_begin * 128;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) gw[q] = g.w + (int64_t)min(n0 + (wave * 4 + q) * 8 + (lane >> 3), g.n - 1) * g.ldw + c * 16 + (int64_t)s_begin * 128;
+  const int8_t* ga = g.a + min(m0 + wave * 8 + (lane >> 3), g.m - 1) * g.lda + c * 16 + (int64_t)s_begin * 128;
+  const int8_t* gw0 = g.w + (int64_t)min(n0 + wave * 16 + (lane >> 3), g.n - 1) * g.ldw + c * 16 + (int64_t)s_begin * 128;
+  const int8_t* gw1 = g.w + (int64_t)min(n0 + wave * 16 + 8 + (lane >> 3), g.n - 1) * g.ldw + c * 16 + (int64_t)s_begin * 128;
   auto issue = [&](int s, int buf) __attribute__((always_inline)) {
     const int back = s == steps - 1 && s * 128 + c * 16 >= g.k ? s * 128 + c * 16 : 0;
-#pragma unroll
-    for (int q = 0; q < QA; ++q) { dma16(ga[q] - back, &lds[buf * STAGE + (wave * QA + q) * 1024]); ga[q] += 128; }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) { dma16(gw[q] - back, &lds[buf * STAGE + BM * 128 + (wave * 4 + q) * 1024]); gw[q] += 128; }
+    dma16(ga - back, &lds[buf * STAGE + wave * 1024]);
+    dma16(gw0 - back, &lds[buf * STAGE + 64 * 128 + wave * 2048]);
+    dma16(gw1 - back, &lds[buf * STAGE + 64 * 128 + wave * 2048 + 1024]);
+    ga += 128; gw0 += 128; gw1 += 128;
   };
-  i32x4_t acc[RI][4];
+  i32x4_t acc[2][4];
 #pragma unroll
-  for (int i = 0; i < RI; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
 #pragma unroll
   for (int st = 0; st < NS - 1; ++st)
     if (st < nk) issue(s_begin + st, st);
+  const int off = (lane & 15) * 128 + (((half * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
   int buf = 0;
   for (int kt = 0; kt < nk; ++kt) {
-    constexpr int PER = QA + 4;                        // requests of a step
-    const int younger = min(NS - 2, nk - 1 - kt);      // steps requested after kt that may stay in flight
-    if (younger >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
-    else if (younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
+    const int younger = min(NS - 2, nk - 1 - kt);      // steps requested after kt (3 requests each) that may stay in flight
+    if (younger >= 4) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    else if (younger == 3) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+    else if (younger == 2) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+    else if (younger == 1) asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // step kt is visible to all; the buffer of step kt - 1 is free (its reads were retired before this barrier)
     q8_barrier();
     if (kt + NS - 1 < nk) issue(s_begin + kt + NS - 1, buf == 0 ? NS - 1 : buf - 1);
-    const int8_t* la = &lds[buf * STAGE];
-    const int8_t* lw = la + BM * 128;
-    i32x4_t af[2][RI], wf[2][4];
+    const int8_t* la = &lds[buf * STAGE + wm * 32 * 128 + off];
+    const int8_t* lw = &lds[buf * STAGE + 64 * 128 + wn * 64 * 128 + off];
+    i32x4_t af[2], wf[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int off = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
+    for (int i = 0; i < 2; ++i) af[i] = *reinterpret_cast<const i32x4_t*>(la + i * 2048);
 #pragma unroll
-      for (int i = 0; i < RI; ++i) af[h][i] = *reinterpret_cast<const i32x4_t*>(&la[(wm * (BM / 2) + i * 16) * 128 + off]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) wf[h][j] = *reinterpret_cast<const i32x4_t*>(&lw[(wn * 64 + j * 16) * 128 + off]);
-    }
+    for (int j = 0; j < 4; ++j) wf[j] = *reinterpret_cast<const i32x4_t*>(lw + j * 2048);
     if (s_begin + kt == steps - 1 && (g.k & 127)) {
+      const i32x4_t mask = piece_mask(g.k - ((s_begin + kt) * 128 + half * 64 + (lane >> 4) * 16));
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const i32x4_t mask = piece_mask(g.k - ((s_begin + kt) * 128 + h * 64 + (lane >> 4) * 16));
-#pragma unroll
-        for (int i = 0; i < RI; ++i) af[h][i] &= mask;
-      }
+      for (int i = 0; i < 2; ++i) af[i] &= mask;
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < RI; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(wf[h][j], af[h][i], acc[i][j]);
+      for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(wf[j], af[i], acc[i][j]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     buf = buf == NS - 1 ? 0 : buf + 1;
   }
-  const int64_t mw = m0 + wm * (BM / 2);
+  // this half finishes rows 16 half .. of the wave's 32 and hands the others over
+  __syncthreads();
+  i32x4_t* swap = reinterpret_cast<i32x4_t*>(lds);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) swap[(wave * 4 + j) * 64 + lane] = half ? acc[0][j] : acc[1][j];
+  __syncthreads();
+  i32x4_t sum[1][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[0][j] = (half ? acc[1][j] : acc[0][j]) + swap[((wave ^ 4) * 4 + j) * 64 + lane];
+  const int64_t mw = m0 + wm * 32 + half * 16;
   const int nw = n0 + wn * 64;
   if (g.ksplit == 1) {
-    q8_epilogue<T, RI>(g, mw, nw, lane, acc);
+    q8_epilogue<T, 1>(g, mw, nw, lane, sum);
     return;
   }
-  int32_t* slab = g.slab + (int64_t)blockIdx.y * g.m * g.n;
+  const int64_t m = mw + (lane & 15);
+  if (m >= g.m) return;
+  int32_t* row = g.slab + ((int64_t)blockIdx.y * g.m + m) * g.n;
 #pragma unroll
-  for (int i = 0; i < RI; ++i) {
-    const int64_t m = mw + i * 16 + (lane & 15);
+  for (int j = 0; j < 4; ++j) {
+    const int n = nw + j * 16 + (lane >> 4) * 4;
+    if (n + 4 <= g.n) __builtin_memcpy(row + n, &sum[0][j], 16);
+    else
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = nw + j * 16 + (lane >> 4) * 4;
-      if (m < g.m) {
-        if (n + 4 <= g.n) __builtin_memcpy(slab + m * g.n + n, &acc[i][j], 16);
-        else
-#pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (n + e < g.n) slab[m * g.n + n + e] = acc[i][j][e];
-      }
-    }
+      for (int e = 0; e < 3; ++e)
+        if (n + e < g.n) row[n + e] = sum[0][j][e];
   }
 }
 
 // out = epilogue of the slices' sums, 4 columns per lane
 template <typename T>
 __global__ __launch_bounds__(256) void q8_gemm_join_kernel(const GemmQ8Args g) {
-  const int groups = (g.n + 3) >> 2;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= g.m * groups) return;
-  const int64_t m = i / groups;
-  const int n = (int)(i - m * groups) * 4;
-  int sum[4] = {0, 0, 0, 0};
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const int64_t m = blockIdx.y;
+  if (n >= g.n) return;
   float sw[4], bias[4] = {0.f, 0.f, 0.f, 0.f};
   ld4_to(g.sw, n, g.n, sw);
   if (g.bias) ld4_to(g.bias, n, g.n, bias);
   const float sa = g.sa[m];
   const bool whole = n + 4 <= g.n;
-  for (int s = 0; s < g.ksplit; ++s) {
-    const int32_t* p = g.slab + ((int64_t)s * g.m + m) * g.n + n;
-    int v[4] = {0, 0, 0, 0};
-    if (whole) __builtin_memcpy(v, p, 16);
-    else
-      for (int e = 0; n + e < g.n; ++e) v[e] = p[e];
+  i32x4_t v[8], sum = i32x4_t{0, 0, 0, 0};             // all slices (at most 8) are requested before the first is added
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += v[e];
+  for (int s = 0; s < 8; ++s) {
+    v[s] = i32x4_t{0, 0, 0, 0};
+    if (s < g.ksplit) {
+      const int32_t* p = g.slab + ((int64_t)s * g.m + m) * g.n + n;
+      if (whole) __builtin_memcpy(&v[s], p, 16);
+      else
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (n + e < g.n) v[s][e] = p[e];
+    }
   }
+#pragma unroll
+  for (int s = 0; s < 8; ++s) sum += v[s];
   T t[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) t[e] = to_T<T>((float)sum[e] * (sa * sw[e]) + bias[e]);
@@ -717,17 +716,16 @@ int launch_rows(wj_ctx* ctx, int dtype, int delta_dtype, const RowArgs& a, void*
 }
 
 // Which kernel a product takes, from its size alone (the workspace follows from it)
-enum GemmKind { GEMM_ROWS, GEMM_BIG, GEMM_TILE128, GEMM_TILE64 };
+enum GemmKind { GEMM_ROWS, GEMM_BIG, GEMM_DEEP, GEMM_TILE };
 struct GemmPlan { GemmKind kind; int ksplit; };
 GemmPlan plan_gemm(int64_t m, int n, int k) {
   if (m <= 64) return {GEMM_ROWS, 1};
-  const int64_t t256 = ((m + 255) / 256) * ((n + 255) / 256), t128 = ((m + 127) / 128) * ((n + 127) / 128), t64 = ((m + 63) / 64) * ((n + 127) / 128);
-  if (t256 >= 192) return {GEMM_BIG, 1};
-  if (t128 >= 256) return {GEMM_TILE128, 1};
+  const int64_t t256 = ((m + 255) / 256) * ((n + 255) / 256), t64 = ((m + 63) / 64) * ((n + 127) / 128);
+  if (t256 >= 160) return {GEMM_BIG, 1};
   const int steps = (k + 127) / 128;
   int ks = 1;
-  while (ks < 8 && t64 * ks * 2 <= 512 && steps >= 4 * ks * 2) ks *= 2;
-  return {GEMM_TILE64, ks};
+  while (ks < 8 && t64 * ks * 2 <= 256 && steps >= 8 * ks) ks *= 2;
+  return {t64 * ks <= 256 ? GEMM_DEEP : GEMM_TILE, ks};
 }
 
 template <typename K>
@@ -739,17 +737,16 @@ int allow_lds(K kernel, AttrOnce& once, int bytes) {
   return WJ_OK;
 }
 
-template <typename T, int BM, int NS>
+template <typename T, int NS>
 int start_tile(const GemmQ8Args& g, hipStream_t s) {
   static AttrOnce once;
-  constexpr int lds = NS * (BM + 128) * 128;
-  if (int rc = allow_lds(q8_gemm_tile_kernel<T, BM, NS>, once, lds)) return rc;
-  const int nx = (g.n + 127) / 128, ny = (int)((g.m + BM - 1) / BM);
-  hipLaunchKernelGGL((q8_gemm_tile_kernel<T, BM, NS>), dim3((unsigned)nx * ny, g.ksplit), dim3(256), lds, s, g, nx, ny);
+  constexpr int lds = NS * (64 + 128) * 128;
+  if (int rc = allow_lds(q8_gemm_tile_kernel<T, NS>, once, lds)) return rc;
+  const int nx = (g.n + 127) / 128, ny = (int)((g.m + 63) / 64);
+  hipLaunchKernelGGL((q8_gemm_tile_kernel<T, NS>), dim3((unsigned)nx * ny, g.ksplit), dim3(512), lds, s, g, nx, ny);
   WJ_LAUNCH_CHECK();
   if (g.ksplit > 1) {
-    const int64_t threads = g.m * ((g.n + 3) / 4);
-    hipLaunchKernelGGL(q8_gemm_join_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL(q8_gemm_join_kernel<T>, dim3((unsigned)((g.n + 1023) / 1024), (unsigned)g.m), dim3(256), 0, s, g);
     WJ_LAUNCH_CHECK();
   }
   return WJ_OK;
@@ -777,8 +774,8 @@ int launch_gemm_q8(GemmQ8Args g, hipStream_t s) {
       WJ_LAUNCH_CHECK();
       return WJ_OK;
     }
-    case GEMM_TILE128: return start_tile<T, 128, 3>(g, s);
-    default: return start_tile<T, 64, 3>(g, s);
+    case GEMM_DEEP: return start_tile<T, 6>(g, s);
+    default: return start_tile<T, 3>(g, s);
   }
 }
 
