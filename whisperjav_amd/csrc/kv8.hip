@@ -1,4 +1,6 @@
 // kv8.hip -- the 8-bit key / value cache: rows quantised as they are written, read back, and the attention over it (gfx950).
+#include <type_traits>
+
 #include "q8.hpp"
 
 using namespace wj;
@@ -64,45 +66,339 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, int dtyp
   }
 }
 
-// One wave per (row, query head): 64 positions at a time, one per lane for the scores, then the dimensions over the lanes for the values.
-__global__ __launch_bounds__(64) void kv8_attention_simple_kernel(const Kv8Args a, int dtype, const void* __restrict__ q, int64_t ldq,
-                                                                  void* __restrict__ out, int64_t ldo, int n_heads, float scale, int causal) {
-  __shared__ float qs[128], ps[64];
-  const Span s = span_of(a, blockIdx.z);
-  const int lane = threadIdx.x, head = blockIdx.y, kvh = head / (n_heads / a.c.heads), dim = a.c.dim;
-  for (int t = blockIdx.x; t < s.n; t += gridDim.x) {
-    const int64_t at = (int64_t)(s.first + t) * ldq + head * dim;
-    __syncthreads();
-    for (int d = lane; d < dim; d += 64) qs[d] = ld_any(q, dtype, at + d) * scale;
-    const int keys = s.slot < 0 ? 0 : min(a.c.ctx, causal ? min(s.len, s.pos0 + t + 1) : s.len);
-    const int64_t row0 = ((int64_t)max(s.slot, 0) * a.c.heads + kvh) * a.c.ctx;
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int base = 0; base < keys; base += 64) {
+// --------------------------------------------------------------------------------------------
+// Attention over the cache.
+//
+// Per key / value head the rows of a sequence are its (new row, query head of the group) pairs, r = t * per + g; a workgroup takes
+// 16 RT of them and a range of positions, its four waves take 32 positions at a time in turn.  Codes go from memory straight into the
+// operands of the matrix cores: S^T = K Q^T per 16 positions, the positions of two such products permuted so that the weights leave the
+// first product in the order the second one, O^T += V^T P^T, wants them.  An int8 code is exact in float16 (byte | 0x6400 is 1024 + byte,
+// minus 1152), so the products lose nothing of the cache; the query is carried in units of a power of two that bounds its row, exact for
+// 16-bit types, as a high and a low half (22 bits) for float32.
+//
+// Weights: with x = scale * log2(e) * ks * (q . k), the numerator of a position is 2^x vs, and 16 bits must hold it whatever the
+// scales are.  So the running reference of a row is M = max(x + exponent of vs), numerators are 2^(x - M) vs (at most 2 times the slack,
+// rounded to float16: 2^-11 of a weight; float32 rows carry high and low halves), the denominator sums 2^(x - M) in float32.  M moves
+// only when it would be exceeded by 2^4.
+// --------------------------------------------------------------------------------------------
+struct AttnArgs {
+  Kv8Args s;
+  const void* q; int64_t ldq;
+  void* out; int64_t ldo;
+  int n_heads, per, causal;
+  float scale2;              // |scale| * log2(e)
+  float sign;                // of scale, goes onto the query
+  int chunk, nsplit;         // positions per workgroup; workgroups per row block (the last takes what is left)
+  float* part;               // nsplit > 1: numerator sums [row * n_heads + head][nsplit][dim]
+  float2* ml;                // ... and (M, denominator)
+};
+
+constexpr float kSlack = 4.f;
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t h2_less(uint32_t w) {      // two halves, 1152 taken off each
+  const h2_t c = {(_Float16)1152.f, (_Float16)1152.f};
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, w) - c);
+}
+// 8 codes of one position -> 8 halves
+__device__ __forceinline__ f16x8_t codes_to_h8(uint32_t a, uint32_t b) {
+  a ^= 0x80808080u; b ^= 0x80808080u;
+  uint4 r;
+  r.x = h2_less(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u));
+  r.y = h2_less(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u));
+  r.z = h2_less(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u));
+  r.w = h2_less(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u));
+  return __builtin_bit_cast(f16x8_t, r);
+}
+// byte E of two positions' words (already ^ 0x80808080) -> two halves
+template <int E> __device__ __forceinline__ uint32_t codes_pair(uint32_t first, uint32_t second) {
+  return h2_less(__builtin_amdgcn_perm(second, first, 0x0c000c00u | ((uint32_t)(4 + E) << 16) | (uint32_t)E) | 0x64006400u);
+}
+
+__device__ __forceinline__ float quad_max(float x) {      // over the four lanes that share lane & 15
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t v = __float_as_uint(x);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+__device__ __forceinline__ float scale_exponent(float vs) {      // of a value scale, bounded so that 2^(x - M) and its sums stay in range
+  return vs == 0.f ? -100.f : fminf(fmaxf((float)__builtin_amdgcn_frexp_expf(vs), -100.f), 110.f);
+}
+
+// the positions that rows r0 .. of a block may see at most, and the row's own
+__device__ __forceinline__ int row_limit(const AttnArgs& a, const Span& s, int r) {
+  if (s.slot < 0) return 0;
+  return max(0, min(a.s.c.ctx, a.causal ? s.pos0 + r / a.per + 1 : s.len));
+}
+
+// The query fragments of row r (this lane's 8 dims of every 32-dim step, see the kernels' dims), in units of 2^ex of its row: NP halves each
+template <typename T, int HD, int NP>
+__device__ __forceinline__ float load_query(const AttnArgs& a, const Span& s, int kvh, int r, int rows, int lg, f16x8_t (&qf)[NP][HD / 32]) {
+  float v[HD / 4], top = 0.f;
+  if (r < rows) {
+    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(s.first + r / a.per) * a.ldq + (int64_t)(kvh * a.per + r % a.per) * HD + lg * (HD / 4);
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c) widen8(ld_raw8(p + c * 8), v + c * 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < HD / 4; ++e) v[e] = 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < HD / 4; ++e) top = fmaxf(top, mag(v[e]));
+  top = quad_max(top);
+  // |v| / unit <= 1; a row that is not finite gets a NaN unit, which makes NaN of its scores alone
+  const int ex = top > 0.f ? max(__builtin_amdgcn_frexp_expf(top), -120) : 0;
+  const float down = ldexpf(a.sign, -ex);
+#pragma unroll
+  for (int c = 0; c < HD / 32; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = top < INFINITY ? v[c * 8 + e] * down : 0.f;
+      const f16_t hi = f2h(x);
+      qf[0][c][e] = hi;
+      if constexpr (NP == 2) qf[1][c][e] = f2h(x - h2f(hi));
+    }
+  return top < INFINITY ? ldexpf(a.scale2, ex) : __uint_as_float(0x7fc00000u);
+}
+
+template <typename T, int N> __device__ __forceinline__ void st_out(T* p, const float* v) {      // any alignment: gfx950 serves wide unaligned stores
+  T t[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) t[e] = to_T<T>(v[e]);
+  __builtin_memcpy(p, t, sizeof(t));
+}
+
+// Parts of one row over different positions, each with its reference and denominator: brought to the largest reference and added.  A part
+// that saw nothing (reference -inf, zeros) adds nothing; one that holds a NaN makes one of the sum.
+template <int N> struct Part {
+  float top = -INFINITY, sum = 0.f, o[N] = {};
+  __device__ __forceinline__ void see(float2 ml) { top = fmaxf(top, ml.x); }
+  __device__ __forceinline__ void add(float2 ml, const float* part) {
+    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
+    sum = fmaf(ml.y, f, sum);
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = fmaf(part[e], f, o[e]);
+  }
+  __device__ __forceinline__ void finish(bool seen) {
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = seen ? o[e] * inv : 0.f;
+  }
+};
+
+template <typename T, int HD, int RT>
+__global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
+  constexpr int NP = sizeof(T) == 4 ? 2 : 1;
+  constexpr int NE = HD / 16;                  // 16-dim tiles of the output; a lane's output dims are NE consecutive ones, four times
+  constexpr int KW = HD / 64;                  // 16-byte pieces of a key per lane
+  constexpr int LDO = HD + 4;
+  __shared__ __attribute__((aligned(16))) float lo[4 * 16 * LDO];
+  __shared__ float2 lml[4 * 16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+  const int kvh = blockIdx.y;
+  const Span s = span_of(a.s, blockIdx.z);
+  const int split = blockIdx.x % a.nsplit, blocks = gridDim.x / a.nsplit;
+  const int64_t rows = (int64_t)s.n * a.per;
+  for (int64_t r0 = (int64_t)(blockIdx.x / a.nsplit) * 16 * RT; r0 < rows; r0 += (int64_t)blocks * 16 * RT) {
+    const int first = (int)r0, last = (int)min(rows, r0 + 16 * RT) - 1;
+    const int every = row_limit(a, s, first), all = row_limit(a, s, last);      // positions that every row / some row of the block sees
+    const int kbeg = split * a.chunk;
+    const int kend = split == a.nsplit - 1 ? all : min(all, kbeg + a.chunk);
+    if (split > 0 && kbeg >= kend) continue;                                    // the join does not read this part
+    const int64_t row0 = ((int64_t)max(s.slot, 0) * a.s.c.heads + kvh) * a.s.c.ctx;
+    const int8_t* kp = a.s.c.k_dev + row0 * HD;
+    const int8_t* vp = a.s.c.v_dev + row0 * HD;
+    const float* ksp = a.s.c.k_scale_dev + row0;
+    const float* vsp = a.s.c.v_scale_dev + row0;
+
+    f16x8_t qf[RT][NP][HD / 32];
+    float unit[RT], M[RT], l[RT];
+    int limit[RT];
+    f32x4_t o[RT][NE];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = first + t * 16 + li;
+      unit[t] = load_query<T, HD, NP>(a, s, kvh, r, (int)rows, lg, qf[t]);
+      limit[t] = r <= last ? min(kend, row_limit(a, s, r)) : kend;
+      M[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    auto tile = [&](const int kt, auto masked_tag) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      // codes of this lane's keys (two rows of K, eight of V) and scales of its eight positions kt + 8 lg ..
+      uint4 kw[2][KW];
+      uint32_t vw[8][HD / 64];
+      float ks[8], vs[8];
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) {
+        int key = kt + 8 * (li >> 2) + 4 * t2 + (li & 3);
+        if (MASKED) key = min(key, kend - 1);
+#pragma unroll
+        for (int c = 0; c < KW; ++c) kw[t2][c] = *reinterpret_cast<const uint4*>(kp + (int64_t)key * HD + lg * (HD / 4) + c * 16);
+      }
+      if (MASKED) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = min(kt + 8 * lg + j, kend - 1);
+          ks[j] = ksp[key]; vs[j] = vsp[key];
+        }
+      } else {
+        __builtin_memcpy(ks, ksp + kt + 8 * lg, 32);
+        __builtin_memcpy(vs, vsp + kt + 8 * lg, 32);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        int key = kt + 8 * lg + j;
+        if (MASKED) key = min(key, kend - 1);
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(vp + (int64_t)key * HD + li * (HD / 16));
+        if constexpr (HD == 128) {
+          const uint2 u = *reinterpret_cast<const uint2*>(src);
+          vw[j][0] = u.x; vw[j][1] = u.y;
+        } else {
+          vw[j][0] = *src;
+        }
+      }
+      float ex[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ex[j] = scale_exponent(vs[j]);
+      f32x4_t st[RT][2];
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) st[t][t2] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KW; ++c) {
+          const f16x8_t k0 = codes_to_h8(kw[t2][c].x, kw[t2][c].y), k1 = codes_to_h8(kw[t2][c].z, kw[t2][c].w);
+#pragma unroll
+          for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+              st[t][t2] = mfma16(k0, qf[t][p][2 * c], st[t][t2]);
+              st[t][t2] = mfma16(k1, qf[t][p][2 * c + 1], st[t][t2]);
+            }
+        }
+      }
+      f16x8_t pf[RT][NP];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        float x[8], top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = st[t][j >> 2][j & 3] * ks[j] * unit[t];
+          const bool in = !MASKED || kt + 8 * lg + j < limit[t];
+          top = fmaxf(top, in ? x[j] + ex[j] : -INFINITY);
+        }
+        top = quad_max(top);
+        if (top > M[t] + kSlack) {
+          const float f = __builtin_amdgcn_exp2f(M[t] - top);      // the first time: 0 on zeros
+          M[t] = top;
+          l[t] *= f;
+#pragma unroll
+          for (int e = 0; e < NE; ++e)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][e][r] *= f;
+        }
+        const float m = M[t] == -INFINITY ? 0.f : M[t];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = !MASKED || kt + 8 * lg + j < limit[t];
+          const float p = in ? __builtin_amdgcn_exp2f(x[j] - m) : 0.f;
+          l[t] += p;
+          const float w = in ? p * vs[j] : 0.f;
+          const f16_t hi = f2h(w);
+          pf[t][0][j] = hi;
+          if constexpr (NP == 2) pf[t][1][j] = f2h(w - h2f(hi));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) vw[j][c] ^= 0x80808080u;
+      auto value_tile = [&](auto e_tag) __attribute__((always_inline)) {
+        constexpr int E = decltype(e_tag)::value, C = E >> 2, B = E & 3;
+        uint4 u;
+        u.x = codes_pair<B>(vw[0][C], vw[1][C]); u.y = codes_pair<B>(vw[2][C], vw[3][C]);
+        u.z = codes_pair<B>(vw[4][C], vw[5][C]); u.w = codes_pair<B>(vw[6][C], vw[7][C]);
+        const f16x8_t vf = __builtin_bit_cast(f16x8_t, u);
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) o[t][E] = mfma16(vf, pf[t][p], o[t][E]);
+      };
+      value_tile(std::integral_constant<int, 0>{}); value_tile(std::integral_constant<int, 1>{});
+      value_tile(std::integral_constant<int, 2>{}); value_tile(std::integral_constant<int, 3>{});
+      if constexpr (HD == 128) {
+        value_tile(std::integral_constant<int, 4>{}); value_tile(std::integral_constant<int, 5>{});
+        value_tile(std::integral_constant<int, 6>{}); value_tile(std::integral_constant<int, 7>{});
+      }
+    };
+    for (int kt = kbeg + 32 * wave; kt < kend; kt += 128) {
+      if (kt + 32 <= min(every, kend)) tile(kt, std::false_type{});
+      else tile(kt, std::true_type{});
+    }
+
+    // the four waves' parts meet in LDS, 16 rows at a time
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if (first + t * 16 > last) break;
       __syncthreads();
-      const bool in = base + lane < keys;
-      const int64_t row = row0 + (in ? base + lane : 0);
-      float dot = 0.f;
-      for (int d = 0; d < dim; ++d) dot = fmaf(qs[d], (float)a.c.k_dev[row * dim + d], dot);
-      const float sc = in ? dot * a.c.k_scale_dev[row] : -INFINITY;
-      const float m_new = fmaxf(m, wave_max(sc));
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = expf(m - m_use), p = in ? expf(sc - m_use) : 0.f;
-      l = l * alpha + wave_sum(p);
-      m = m_new;
-      ps[lane] = in ? p * a.c.v_scale_dev[row] : 0.f;
+      const float lsum = quad_sum(l[t]);
+      if (lg == 0) lml[wave * 16 + li] = make_float2(M[t], lsum);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float* d = &lo[(wave * 16 + li) * LDO + NE * (4 * lg + r)];
+#pragma unroll
+        for (int e = 0; e < NE; e += 4) *reinterpret_cast<float4*>(d + e) = make_float4(o[t][e][r], o[t][e + 1][r], o[t][e + 2][r], o[t][e + 3][r]);
+      }
       __syncthreads();
-      o0 *= alpha; o1 *= alpha;
-      const int n = min(64, keys - base);
-      for (int j = 0; j < n; ++j) {
-        const int8_t* vr = a.c.v_dev + (row0 + base + j) * dim;
-        o0 = fmaf(ps[j], (float)vr[lane], o0);
-        if (dim == 128) o1 = fmaf(ps[j], (float)vr[64 + lane], o1);
+      const int row = tid >> 4, r = first + t * 16 + row, d0 = (tid & 15) * NE;
+      if (r <= last) {
+        Part<NE> p;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) p.see(lml[w * 16 + row]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) p.add(lml[w * 16 + row], &lo[(w * 16 + row) * LDO + d0]);
+        const int64_t at = (int64_t)(s.first + r / a.per), head = kvh * a.per + r % a.per;
+        if (a.nsplit == 1) {
+          p.finish(row_limit(a, s, r) > 0);
+          st_out<T, NE>(reinterpret_cast<T*>(a.out) + at * a.ldo + head * HD + d0, p.o);
+        } else {
+          const int64_t slot = (at * a.n_heads + head) * a.nsplit + split;
+          if ((tid & 15) == 0) a.ml[slot] = make_float2(p.top, p.sum);
+#pragma unroll
+          for (int e = 0; e < NE; e += 4) *reinterpret_cast<float4*>(a.part + slot * HD + d0 + e) = make_float4(p.o[e], p.o[e + 1], p.o[e + 2], p.o[e + 3]);
+        }
       }
     }
-    const int64_t to = (int64_t)(s.first + t) * ldo + head * dim;
-    const float inv = keys > 0 ? 1.f / l : 0.f;
-    st_any(out, dtype, to + lane, keys > 0 ? o0 * inv : 0.f);
-    if (dim == 128) st_any(out, dtype, to + 64 + lane, keys > 0 ? o1 * inv : 0.f);
+  }
+}
+
+// The parts of every row's positions joined, in order: 16 lanes per (row, head)
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void kv8_attn_join_kernel(const AttnArgs a, int block_rows) {
+  constexpr int NE = HD / 16;
+  const Span s = span_of(a.s, blockIdx.y);
+  const int d0 = (threadIdx.x & 15) * NE;
+  const int total = s.n * a.n_heads;
+  for (int i = blockIdx.x * 16 + (threadIdx.x >> 4); i < total; i += gridDim.x * 16) {
+    const int t = i / a.n_heads, head = i - t * a.n_heads, r = t * a.per + head % a.per;
+    const int last = min(s.n * a.per, (r / block_rows + 1) * block_rows) - 1;         // of the row's block: its workgroups went by that limit
+    const int parts = min(a.nsplit, max(1, (row_limit(a, s, last) + a.chunk - 1) / a.chunk));
+    const int64_t slot = ((int64_t)(s.first + t) * a.n_heads + head) * a.nsplit;
+    Part<NE> p;
+    for (int j = 0; j < parts; ++j) p.see(a.ml[slot + j]);
+    for (int j = 0; j < parts; ++j) p.add(a.ml[slot + j], a.part + (slot + j) * HD + d0);
+    p.finish(row_limit(a, s, r) > 0);
+    st_out<T, NE>(reinterpret_cast<T*>(a.out) + (int64_t)(s.first + t) * a.ldo + head * HD + d0, p.o);
   }
 }
 
@@ -119,6 +415,47 @@ int check_kv8(const char* who, wj_ctx* ctx, const wj_kv8* c, const wj_kv8_batch*
   WJ_REQUIRE(aligned_to(c->k_dev, 16) && aligned_to(c->v_dev, 16) && aligned_to(c->k_scale_dev, 4) && aligned_to(c->v_scale_dev, 4),
              "%s: the cache's codes are not 16-byte aligned (scales: 4)", who);
   return WJ_OK;
+}
+
+// Rows per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).
+struct AttnPlan { int rt, nsplit, chunk; };
+AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
+  const int per = n_heads / c.heads;
+  const int64_t rows = (int64_t)(b.max_new > 0 ? b.max_new : 1) * per;
+  AttnPlan p;
+  p.rt = rows <= 16 ? 1 : 2;
+  const int64_t groups = (int64_t)b.seqs * c.heads * ((rows + 16 * p.rt - 1) / (16 * p.rt));
+  const int len = b.max_len < c.ctx ? (b.max_len > 0 ? b.max_len : 1) : c.ctx;
+  const int64_t want = groups >= 1024 ? 1 : (1024 + groups - 1) / groups;                // workgroups of four waves, four per CU
+  const int most = (len + 127) / 128;                                                    // a wave's turn is 32 positions
+  const int n = (int)(want < most ? want : most);
+  p.chunk = ((len + n - 1) / n + 127) / 128 * 128;
+  p.nsplit = (len + p.chunk - 1) / p.chunk;
+  return p;
+}
+
+template <typename T, int HD, int RT>
+int start_attention(const AttnArgs& a, hipStream_t s) {
+  const int64_t rows = (int64_t)(a.s.b.max_new > 0 ? a.s.b.max_new : 1) * a.per;
+  const int64_t blocks = (rows + 16 * RT - 1) / (16 * RT);
+  hipLaunchKernelGGL((kv8_attn_rows_kernel<T, HD, RT>), dim3((unsigned)(blocks * a.nsplit), a.s.c.heads, a.s.b.seqs), dim3(256), 0, s, a);
+  WJ_LAUNCH_CHECK();
+  if (a.nsplit > 1) {
+    const int64_t groups = ((int64_t)(a.s.b.max_new > 0 ? a.s.b.max_new : 1) * a.n_heads + 15) / 16;
+    hipLaunchKernelGGL((kv8_attn_join_kernel<T, HD>), dim3((unsigned)groups, a.s.b.seqs), dim3(256), 0, s, a, 16 * RT);
+    WJ_LAUNCH_CHECK();
+  }
+  return WJ_OK;
+}
+template <int HD, typename T>
+int pick_rows(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+  return p.rt == 1 ? start_attention<T, HD, 1>(a, s) : start_attention<T, HD, 2>(a, s);
+}
+template <int HD>
+int pick_type(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t s) {
+  if (dtype == WJ_F32) return pick_rows<HD, float>(a, p, s);
+  if (dtype == WJ_F16) return pick_rows<HD, f16_t>(a, p, s);
+  return pick_rows<HD, bf16_t>(a, p, s);
 }
 
 }  // namespace
@@ -157,8 +494,10 @@ int wj_kv8_read(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int
 }
 
 int64_t wj_kv8_attention_workspace(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int n_heads) {
-  (void)ctx; (void)cache; (void)batch; (void)n_heads;
-  return 0;
+  (void)ctx;
+  if (!cache || !batch || batch->seqs <= 0 || batch->rows <= 0 || n_heads <= 0 || cache->heads <= 0 || n_heads % cache->heads) return 0;
+  const AttnPlan p = plan_attention(*cache, *batch, n_heads);
+  return p.nsplit > 1 ? (int64_t)batch->rows * n_heads * p.nsplit * (cache->dim * 4 + 8) : 0;
 }
 
 int wj_kv8_attention(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int dtype, const void* q_dev, int64_t ldq, void* out_dev,
@@ -169,15 +508,20 @@ int wj_kv8_attention(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch
   if (batch->seqs == 0 || batch->rows == 0) return WJ_OK;
   WJ_REQUIRE((int64_t)cache->slots * cache->ctx > 0, "wj_kv8_attention: an empty cache");
   WJ_REQUIRE(q_dev && out_dev, "wj_kv8_attention: NULL argument");
-  WJ_REQUIRE(ldq >= 0 && (batch->rows == 1 || ldo >= n_heads * cache->dim), "wj_kv8_attention: output rows overlap");
-  WJ_REQUIRE(workspace_bytes >= wj_kv8_attention_workspace(ctx, cache, batch, n_heads), "wj_kv8_attention: workspace too small");
+  WJ_REQUIRE((int64_t)batch->rows * n_heads < ((int64_t)1 << 31) - 4096, "wj_kv8_attention: %d rows of %d heads", batch->rows, n_heads);
+  WJ_REQUIRE(ldq >= 0 && (batch->rows == 1 || ldo >= (int64_t)n_heads * cache->dim), "wj_kv8_attention: output rows overlap");
+  const int64_t need = wj_kv8_attention_workspace(ctx, cache, batch, n_heads);
+  WJ_REQUIRE(workspace_bytes >= need && (workspace_dev || need == 0), "wj_kv8_attention: %lld bytes of workspace, %lld needed", (long long)workspace_bytes, (long long)need);
+  WJ_REQUIRE(aligned_to(workspace_dev, 16), "wj_kv8_attention: the workspace is not 16-byte aligned");
   DeviceScope dev;
   WJ_HIP(dev.enter(ctx->device));
-  (void)workspace_dev;
-  hipLaunchKernelGGL(kv8_attention_simple_kernel, dim3(batch->max_new > 0 ? batch->max_new : 1, n_heads, batch->seqs), dim3(64), 0, ctx->pick(stream),
-                     Kv8Args{*cache, *batch}, dtype, q_dev, ldq, out_dev, ldo, n_heads, scale, causal);
-  WJ_LAUNCH_CHECK();
-  return WJ_OK;
+  const AttnPlan p = plan_attention(*cache, *batch, n_heads);
+  AttnArgs a{Kv8Args{*cache, *batch}, q_dev, ldq, out_dev, ldo, n_heads, n_heads / cache->heads, causal, fabsf(scale) * 1.44269504088896340736f,
+             scale < 0.f ? -1.f : 1.f, p.chunk, p.nsplit, reinterpret_cast<float*>(workspace_dev), nullptr};
+  a.ml = reinterpret_cast<float2*>(a.part + (int64_t)batch->rows * n_heads * p.nsplit * cache->dim);
+  hipStream_t s = ctx->pick(stream);
+  if (cache->dim == 128) return pick_type<128>(a, p, dtype, s);
+  return pick_type<64>(a, p, dtype, s);
 }
 
 }  // extern "C"

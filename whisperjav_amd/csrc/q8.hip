@@ -30,31 +30,6 @@ enum RowMode { ROW_NORM, ROW_PLAIN, ROW_SWIGLU };
 struct NoType {};                              // "no delta"
 constexpr int kSteps = 4;
 
-template <typename T> struct Raw8 { uint32_t w[8 * sizeof(T) / 4]; };      // 8 elements as they lie in memory
-template <typename T> __device__ __forceinline__ Raw8<T> ld_raw8(const T* p) {
-  Raw8<T> r;
-  __builtin_memcpy(&r, p, sizeof(r));
-  return r;
-}
-__device__ __forceinline__ void widen8(const Raw8<float>& r, float v[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r.w[e]);
-}
-__device__ __forceinline__ void widen8(const Raw8<f16_t>& r, float v[8]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) unpack2<f16_t>(r.w[e], v[2 * e], v[2 * e + 1]);
-}
-__device__ __forceinline__ void widen8(const Raw8<bf16_t>& r, float v[8]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) unpack2<bf16_t>(r.w[e], v[2 * e], v[2 * e + 1]);
-}
-template <typename T> __device__ __forceinline__ void st8(T* p, const float v[8]) {
-  T t[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) t[e] = to_T<T>(v[e]);
-  __builtin_memcpy(p, t, sizeof(t));
-}
-
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
 
 template <int WPR> __device__ __forceinline__ float row_sum(float v, float* part) {
@@ -447,14 +422,14 @@ __global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, in
   q8_epilogue<T, 8>(g, m0 + wm * 128, n0 + wn * 64, lane, acc);
 }
 
-// 64 x 128 tile, k steps of 128 codes, a ring of NS buffers with NS - 1 steps requested ahead.  Eight waves: (2 x 2, 32 x 64 each) twice,
+// 64 x 128 tile, k steps of 128 codes, a ring of 3 buffers with 2 steps requested ahead, two workgroups per CU.  Eight waves: (2 x 2, 32 x 64 each) twice,
 // each four taking one half of every step's codes, so that the two waves of a SIMD overlap one's LDS reads with the other's products; the
 // two halves' sums meet in LDS at the end, each four finishing 16 of every 32 rows.  For calls with too few 256-tiles to fill the chip;
 // ksplit > 1: slices of k on the grid's second axis write raw sums, joined by q8_gemm_join_kernel.
-template <typename T, int NS>
+template <typename T>
 __global__ __launch_bounds__(512) void q8_gemm_tile_kernel(const GemmQ8Args g, int nx, int ny) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [stage][A: 64 | W: 128][128]
-  constexpr int STAGE = (64 + 128) * 128;
+  constexpr int NS = 3, STAGE = (64 + 128) * 128;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
@@ -488,10 +463,7 @@ __global__ __launch_bounds__(512) void q8_gemm_tile_kernel(const GemmQ8Args g, i
   int buf = 0;
   for (int kt = 0; kt < nk; ++kt) {
     const int younger = min(NS - 2, nk - 1 - kt);      // steps requested after kt (3 requests each) that may stay in flight
-    if (younger >= 4) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
-    else if (younger == 3) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
-    else if (younger == 2) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-    else if (younger == 1) asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
+    if (younger >= 1) asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // step kt is visible to all; the buffer of step kt - 1 is free (its reads were retired before this barrier)
     q8_barrier();
@@ -715,17 +687,24 @@ int launch_rows(wj_ctx* ctx, int dtype, int delta_dtype, const RowArgs& a, void*
   return pick_delta<MODE, bf16_t>(a, delta_dtype, s);
 }
 
-// Which kernel a product takes, from its size alone (the workspace follows from it)
-enum GemmKind { GEMM_ROWS, GEMM_BIG, GEMM_DEEP, GEMM_TILE };
+// Which kernel a product takes, from its size alone (the workspace follows from it).  Measured on the MI355X, us per call in a graph:
+//   rows / tile: 16 x 5176 x 5824 10.3 / 11.5, 48 x 4096 x 2048 6.3 / 8.6, 64 x 4096 x 2048 7.1 / 9.4, 64 x 12288 x 2048 17.0 / 10.3,
+//     32 x 5176 x 5824 14.2 / 11.8: the rows kernel reads the activations once per 16 columns, so beyond 16 rows it is for products where
+//     that is at most 36 MiB;
+//   tile / big: 2048 x 4096 x 2048 27.6 / 29.6, 3000 x 2048 x 6144 53 / 67, 512 x 12288 x 2048 22 / 30, 1024 x 12288 x 2048 40 / 32,
+//     3000 x 4096 x 2048 39 / 31, 1500 x 12288 x 2048 58 / 58: a round of 256 big tiles, filled or not, takes as long as 1000 small ones;
+//   tile, slices 1 / 2 / 4: 100 x 4096 x 2048 10.0 / 11.1 / 11.6, 100 x 2048 x 6144 23 / 15 / 12.5, 512 x 2048 x 6144 22.5 / 19.1 / 19.8: a
+//     slice saves its share of the 0.4 us that a step takes and the join costs 3 us, so it pays from 16 steps a slice while CUs are idle.
+enum GemmKind { GEMM_ROWS, GEMM_BIG, GEMM_TILE };
 struct GemmPlan { GemmKind kind; int ksplit; };
 GemmPlan plan_gemm(int64_t m, int n, int k) {
-  if (m <= 64) return {GEMM_ROWS, 1};
+  if (m <= 16 || (m <= 64 && m * k * ((n + 15) / 16) <= (int64_t)36 << 20)) return {GEMM_ROWS, 1};
   const int64_t t256 = ((m + 255) / 256) * ((n + 255) / 256), t64 = ((m + 63) / 64) * ((n + 127) / 128);
-  if (t256 >= 160) return {GEMM_BIG, 1};
+  if (t64 > 1000 * ((t256 + 255) / 256)) return {GEMM_BIG, 1};
   const int steps = (k + 127) / 128;
   int ks = 1;
-  while (ks < 8 && t64 * ks * 2 <= 256 && steps >= 8 * ks) ks *= 2;
-  return {t64 * ks <= 256 ? GEMM_DEEP : GEMM_TILE, ks};
+  while (ks < 8 && t64 * ks * 2 <= 256 && steps > 16 * ks) ks *= 2;
+  return {GEMM_TILE, ks};
 }
 
 template <typename K>
@@ -737,13 +716,13 @@ int allow_lds(K kernel, AttrOnce& once, int bytes) {
   return WJ_OK;
 }
 
-template <typename T, int NS>
+template <typename T>
 int start_tile(const GemmQ8Args& g, hipStream_t s) {
   static AttrOnce once;
-  constexpr int lds = NS * (64 + 128) * 128;
-  if (int rc = allow_lds(q8_gemm_tile_kernel<T, NS>, once, lds)) return rc;
+  constexpr int lds = 3 * (64 + 128) * 128;
+  if (int rc = allow_lds(q8_gemm_tile_kernel<T>, once, lds)) return rc;
   const int nx = (g.n + 127) / 128, ny = (int)((g.m + 63) / 64);
-  hipLaunchKernelGGL((q8_gemm_tile_kernel<T, NS>), dim3((unsigned)nx * ny, g.ksplit), dim3(512), lds, s, g, nx, ny);
+  hipLaunchKernelGGL((q8_gemm_tile_kernel<T>), dim3((unsigned)nx * ny, g.ksplit), dim3(512), lds, s, g, nx, ny);
   WJ_LAUNCH_CHECK();
   if (g.ksplit > 1) {
     hipLaunchKernelGGL(q8_gemm_join_kernel<T>, dim3((unsigned)((g.n + 1023) / 1024), (unsigned)g.m), dim3(256), 0, s, g);
@@ -774,8 +753,7 @@ int launch_gemm_q8(GemmQ8Args g, hipStream_t s) {
       WJ_LAUNCH_CHECK();
       return WJ_OK;
     }
-    case GEMM_DEEP: return start_tile<T, 6>(g, s);
-    default: return start_tile<T, 3>(g, s);
+    default: return start_tile<T>(g, s);
   }
 }
 

@@ -65,6 +65,32 @@ struct RowQuant {
   }
 };
 
+// 8 consecutive elements, at any alignment: gfx950 serves wide unaligned accesses
+template <typename T> struct Raw8 { uint32_t w[8 * sizeof(T) / 4]; };      // 8 elements as they lie in memory
+template <typename T> __device__ __forceinline__ Raw8<T> ld_raw8(const T* p) {
+  Raw8<T> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+__device__ __forceinline__ void widen8(const Raw8<float>& r, float v[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r.w[e]);
+}
+__device__ __forceinline__ void widen8(const Raw8<f16_t>& r, float v[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) unpack2<f16_t>(r.w[e], v[2 * e], v[2 * e + 1]);
+}
+__device__ __forceinline__ void widen8(const Raw8<bf16_t>& r, float v[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) unpack2<bf16_t>(r.w[e], v[2 * e], v[2 * e + 1]);
+}
+template <typename T> __device__ __forceinline__ void st8(T* p, const float v[8]) {
+  T t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = to_T<T>(v[e]);
+  __builtin_memcpy(p, t, sizeof(t));
+}
+
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
   return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) | ((uint32_t)d << 24);
 }
