@@ -77,9 +77,11 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, int dtyp
 // 16-bit types, as a high and a low half (22 bits) for float32.
 //
 // Weights: with x = scale * log2(e) * ks * (q . k), the numerator of a position is 2^x vs, and 16 bits must hold it whatever the
-// scales are.  So the running reference of a row is M = max(x + exponent of vs), numerators are 2^(x - M) vs (at most 2 times the slack,
-// rounded to float16: 2^-11 of a weight; float32 rows carry high and low halves), the denominator sums 2^(x - M) in float32.  M moves
-// only when it would be exceeded by 2^4.
+// scales are.  So the running reference of a row is M = max(x + exponent of vs), numerators are 2^(x - M) vs (at most 2^4, the slack), the
+// denominator sums 2^(x - M) in float32.  M moves only when it would be exceeded by 2^4.  A numerator goes into the product as one half
+// for bfloat16 rows (2^-12 of a weight, an eighth of what rounding the output costs) and as a high and a low half (22 bits) for float16
+// and float32 rows: with one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 (512 sequences; 124 us either way, the
+// matrix pipe has room).
 // --------------------------------------------------------------------------------------------
 struct AttnArgs {
   Kv8Args s;
@@ -195,7 +197,8 @@ template <int N> struct Part {
 
 template <typename T, int HD, int RT>
 __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
-  constexpr int NP = sizeof(T) == 4 ? 2 : 1;
+  constexpr int NP = sizeof(T) == 4 ? 2 : 1;                              // halves of a query
+  constexpr int NW = std::is_same<T, bf16_t>::value ? 1 : 2;              // halves of a weight
   constexpr int NE = HD / 16;                  // 16-dim tiles of the output; a lane's output dims are NE consecutive ones, four times
   constexpr int KW = HD / 64;                  // 16-byte pieces of a key per lane
   constexpr int LDO = HD + 4;
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
             }
         }
       }
-      f16x8_t pf[RT][NP];
+      f16x8_t pf[RT][NW];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         float x[8], top = -INFINITY;
@@ -316,7 +319,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
           const float w = in ? p * vs[j] : 0.f;
           const f16_t hi = f2h(w);
           pf[t][0][j] = hi;
-          if constexpr (NP == 2) pf[t][1][j] = f2h(w - h2f(hi));
+          if constexpr (NW == 2) pf[t][1][j] = f2h(w - h2f(hi));
         }
       }
 #pragma unroll
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int p = 0; p < NP; ++p) o[t][E] = mfma16(vf, pf[t][p], o[t][E]);
+          for (int p = 0; p < NW; ++p) o[t][E] = mfma16(vf, pf[t][p], o[t][E]);
       };
       value_tile(std::integral_constant<int, 0>{}); value_tile(std::integral_constant<int, 1>{});
       value_tile(std::integral_constant<int, 2>{}); value_tile(std::integral_constant<int, 3>{});

@@ -28,7 +28,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import hipbind
-from .hipbind import WJ_BF16, WJ_F16, WJ_F32, WjError
+from .hipbind import WJ_BF16, WJ_F16, WJ_F32
 
 _TYPE = {torch.float32: WJ_F32, torch.float16: WJ_F16, torch.bfloat16: WJ_BF16}
 _STREAM_DEFAULT = C.c_void_p(-1)        # include/wjhip.h: WJ_STREAM_DEFAULT
@@ -44,44 +44,48 @@ class Kv8BatchC(C.Structure):
                 ("seqs", C.c_int32), ("rows", C.c_int32), ("max_new", C.c_int32), ("max_len", C.c_int32)]
 
 
-def _launch(device: torch.device):
-    """(library, context handle, stream) for tensors on ``device``."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    return hipbind.lib(), hipbind.context(device.index).handle, C.c_void_p(stream) if stream else _STREAM_DEFAULT
+def _launch(index: int):
+    """(library, context handle, stream) for tensors on GPU ``index``.  The calls of a decode step are bound by the host: the raw stream
+    handle costs 0.1 us where a ``torch.cuda.Stream`` object costs 2."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    return hipbind.lib(), hipbind.context(index).handle, stream or _STREAM_DEFAULT
 
 
-def _done(rc: int, name: str) -> None:
-    if rc:
-        hipbind.check(rc, name)
+def _fail(name: str, rc: int) -> None:
+    hipbind.check(rc, name)
 
 
-def _rows(t: torch.Tensor, what: str, device: Optional[torch.device] = None, shape: Optional[Tuple[int, int]] = None) -> int:
-    """Check a ``[rows, cols]`` float tensor whose rows are contiguous; its type code."""
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{what}: {'[rows, cols]' if shape is None else list(shape)} expected, got {list(t.shape)}")
-    if t.dtype not in _TYPE:
+def _float_rows(t: torch.Tensor, what: str, index: Optional[int] = None, rows: int = -1, cols: int = -1) -> int:
+    """Check a ``[rows, cols]`` float tensor whose rows are contiguous (on GPU ``index``); its type code."""
+    code = _TYPE.get(t.dtype)
+    if code is None:
         raise ValueError(f"{what}: float32, float16 or bfloat16 expected, got {t.dtype}")
-    _place(t, what, device)
-    return _TYPE[t.dtype]
+    shape = t.shape
+    if len(shape) != 2 or (index is not None and (shape[0] != rows or shape[1] != cols)):
+        raise ValueError(f"{what}: {'[rows, cols]' if index is None else [rows, cols]} expected, got {list(shape)}")
+    if not t.is_cuda or (index is not None and t.get_device() != index):
+        raise ValueError(f"{what}: on {t.device}, expected {'a GPU' if index is None else f'cuda:{index}'}")
+    if t.stride(1) != 1 and shape[1] > 1:
+        raise ValueError(f"{what}: the elements of a row must be contiguous (stride {t.stride(1)})")
+    return code
 
 
-def _place(t: torch.Tensor, what: str, device: Optional[torch.device] = None) -> None:
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise ValueError(f"{what}: on {t.device}, expected {'a GPU' if device is None else device}")
-    if t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{what}: the elements of a row must be contiguous (stride {t.stride(-1)})")
-
-
-def _codes(t: torch.Tensor, scale: torch.Tensor, what: str, device: Optional[torch.device] = None) -> None:
-    if t.dim() != 2 or t.dtype != torch.int8:
+def _codes(t: torch.Tensor, scale: torch.Tensor, what: str, index: Optional[int] = None) -> int:
+    """Check int8 rows and their scales; the GPU's index."""
+    if t.dtype != torch.int8 or t.dim() != 2:
         raise ValueError(f"{what}: int8 [rows, cols] expected, got {t.dtype} {list(t.shape)}")
-    _place(t, what, device)
-    _vector(scale, f"{what} scale", t.shape[0], t.device)
+    if not t.is_cuda or (index is not None and t.get_device() != index):
+        raise ValueError(f"{what}: on {t.device}, expected {'a GPU' if index is None else f'cuda:{index}'}")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise ValueError(f"{what}: the elements of a row must be contiguous (stride {t.stride(1)})")
+    index = t.get_device()
+    _vector(scale, what + " scale", t.shape[0], index)
+    return index
 
 
-def _vector(t: torch.Tensor, what: str, n: int, device: torch.device) -> None:
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what}: contiguous float32 [{n}] on {device} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+def _vector(t: torch.Tensor, what: str, n: int, index: int) -> None:
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or t.get_device() != index:
+        raise ValueError(f"{what}: contiguous float32 [{n}] on cuda:{index} expected, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _output(t: torch.Tensor, what: str) -> None:
@@ -101,53 +105,60 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, delta: 
     """``(codes, scale)`` of the rows of ``(x + delta) / rms(x + delta) * weight``.
 
     ``residual`` receives ``x + delta`` in x's type; left out, the sum is written back into ``x`` (when there is a ``delta``)."""
-    xt = _rows(x, "x")
+    xt = _float_rows(x, "x")
     rows, cols = x.shape
-    _vector(weight, "weight", cols, x.device)
-    dt = 0
-    if delta is not None:
-        dt = _rows(delta, "delta", x.device, (rows, cols))
+    index = x.get_device()
+    _vector(weight, "weight", cols, index)
+    if delta is None:
+        dt, dp, ld = 0, None, 0
+    else:
+        dt, dp, ld = _float_rows(delta, "delta", index, rows, cols), delta.data_ptr(), delta.stride(0)
+        if residual is None:
+            residual = x
     if residual is None:
-        residual = x if delta is not None else None
-    elif _rows(residual, "residual", x.device, (rows, cols)) != xt:
-        raise ValueError(f"residual: {x.dtype} expected, got {residual.dtype}")
-    if residual is not None:
+        rp, lr = None, 0
+    else:
+        if _float_rows(residual, "residual", index, rows, cols) != xt:
+            raise ValueError(f"residual: {x.dtype} expected, got {residual.dtype}")
         _output(residual, "residual")
+        rp, lr = residual.data_ptr(), residual.stride(0)
     codes, scale = _new_codes(rows, cols, x.device)
-    lib, ctx, stream = _launch(x.device)
-    _done(lib.wj_q8_rmsnorm(ctx, xt, x.data_ptr(), x.stride(0), dt, delta.data_ptr() if delta is not None else None,
-                            delta.stride(0) if delta is not None else 0, weight.data_ptr(), eps,
-                            residual.data_ptr() if residual is not None else None, residual.stride(0) if residual is not None else 0,
-                            codes.data_ptr(), codes.stride(0), scale.data_ptr(), rows, cols, stream), "wj_q8_rmsnorm")
+    lib, ctx, stream = _launch(index)
+    rc = lib.wj_q8_rmsnorm(ctx, xt, x.data_ptr(), x.stride(0), dt, dp, ld, weight.data_ptr(), eps, rp, lr, codes.data_ptr(), codes.stride(0),
+                           scale.data_ptr(), rows, cols, stream)
+    if rc:
+        _fail("wj_q8_rmsnorm", rc)
     return codes, scale
 
 
 def quantize(x: torch.Tensor, *, swiglu_block: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scale)`` of the rows of ``x``, or of ``silu(gate) * up`` where ``x`` holds gate and up columns in alternating blocks of
     ``swiglu_block`` (half of x's columns: ``[gate | up]``; 16: the engine's packed gate-up rows)."""
-    xt = _rows(x, "x")
+    xt = _float_rows(x, "x")
     rows, cols = x.shape
     if swiglu_block:
         if swiglu_block < 0 or cols % (2 * swiglu_block):
             raise ValueError(f"x: {cols} columns are no whole number of gate / up blocks of {swiglu_block}")
         cols //= 2
     codes, scale = _new_codes(rows, cols, x.device)
-    lib, ctx, stream = _launch(x.device)
-    _done(lib.wj_q8_quantize(ctx, xt, x.data_ptr(), x.stride(0), swiglu_block, codes.data_ptr(), codes.stride(0), scale.data_ptr(), rows, cols,
-                             stream), "wj_q8_quantize")
+    lib, ctx, stream = _launch(x.get_device())
+    rc = lib.wj_q8_quantize(ctx, xt, x.data_ptr(), x.stride(0), swiglu_block, codes.data_ptr(), codes.stride(0), scale.data_ptr(), rows, cols, stream)
+    if rc:
+        _fail("wj_q8_quantize", rc)
     return codes, scale
 
 
 def dequantize(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
     """``codes * scale`` in ``dtype``."""
-    _codes(codes, scale, "codes")
+    index = _codes(codes, scale, "codes")
     if dtype not in _TYPE:
         raise ValueError(f"dtype: float32, float16 or bfloat16 expected, got {dtype}")
     rows, cols = codes.shape
     out = torch.empty((rows, cols), dtype=dtype, device=codes.device)
-    lib, ctx, stream = _launch(codes.device)
-    _done(lib.wj_q8_dequantize(ctx, codes.data_ptr(), codes.stride(0), scale.data_ptr(), _TYPE[dtype], out.data_ptr(), cols, rows, cols, stream),
-          "wj_q8_dequantize")
+    lib, ctx, stream = _launch(index)
+    rc = lib.wj_q8_dequantize(ctx, codes.data_ptr(), codes.stride(0), scale.data_ptr(), _TYPE[dtype], out.data_ptr(), cols, rows, cols, stream)
+    if rc:
+        _fail("wj_q8_dequantize", rc)
     return out
 
 
@@ -157,35 +168,42 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
 
     ``a`` int8 ``[m, k]``, ``w`` int8 ``[n, k]``; rows that start at multiples of 16 bytes (what ``rmsnorm`` / ``quantize`` return) take the
     fast kernels."""
-    _codes(a, a_scale, "a")
-    _codes(w, w_scale, "w", a.device)
+    index = _codes(a, a_scale, "a")
+    _codes(w, w_scale, "w", index)
     (m, k), n = a.shape, w.shape[0]
     if w.shape[1] != k:
         raise ValueError(f"a has {k} columns, w has {w.shape[1]}")
     if bias is not None:
-        _vector(bias, "bias", n, a.device)
+        _vector(bias, "bias", n, index)
     if out is None:
-        if dtype not in _TYPE:
+        dt = _TYPE.get(dtype)
+        if dt is None:
             raise ValueError(f"dtype: float32, float16 or bfloat16 expected, got {dtype}")
         out = torch.empty((m, n), dtype=dtype, device=a.device)
     else:
-        _rows(out, "out", a.device, (m, n))
+        dt = _float_rows(out, "out", index, m, n)
         _output(out, "out")
-    lib, ctx, stream = _launch(a.device)
+    lib, ctx, stream = _launch(index)
     need = lib.wj_q8_gemm_workspace(ctx, m, n, k)
-    work = torch.empty((need,), dtype=torch.uint8, device=a.device) if need else None
-    _done(lib.wj_q8_gemm(ctx, a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0), w_scale.data_ptr(),
-                         bias.data_ptr() if bias is not None else None, _TYPE[out.dtype], out.data_ptr(), out.stride(0), m, n, k,
-                         work.data_ptr() if work is not None else None, need, stream), "wj_q8_gemm")
+    work = torch.empty((need,), dtype=torch.uint8, device=a.device) if need else None      # freed in stream order by torch's allocator
+    rc = lib.wj_q8_gemm(ctx, a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0), w_scale.data_ptr(),
+                        bias.data_ptr() if bias is not None else None, dt, out.data_ptr(), out.stride(0), m, n, k,
+                        work.data_ptr() if need else None, need, stream)
+    if rc:
+        _fail("wj_q8_gemm", rc)
     return out
 
 
-class KV8Cache(NamedTuple):
-    """One layer's keys and values in 8 bits: codes int8 ``[slots, heads, ctx, dim]`` and scales float32 ``[slots, heads, ctx]``."""
+class _CacheTensors(NamedTuple):
     k: torch.Tensor
     k_scale: torch.Tensor
     v: torch.Tensor
     v_scale: torch.Tensor
+
+
+class KV8Cache(_CacheTensors):
+    """One layer's keys and values in 8 bits: codes int8 ``[slots, heads, ctx, dim]`` and scales float32 ``[slots, heads, ctx]``.
+    A program keeps it like a handle: the tensors are checked at its first use, and their memory has to stay where it is."""
 
     @classmethod
     def empty(cls, slots: int, heads: int, ctx: int, dim: int, device: torch.device = torch.device("cuda", 0)) -> "KV8Cache":
@@ -197,11 +215,7 @@ class KV8Cache(NamedTuple):
         return cls(codes(), scale(), codes(), scale())
 
 
-class Batch(NamedTuple):
-    """The sequences of a call, int32 on the device: sequence b owns rows ``starts[b] .. starts[b + 1] - 1`` of the row tensors and has
-    ``lens[b]`` positions in slot ``slots[b]`` of the cache once they are written, the rows being the last ones.  A slot of -1 is padding.
-    ``max_new`` / ``max_len``: the most new rows / positions of any sequence; they size the launch (results do not depend on them).  The
-    arrays may change between replays of a captured graph.  Slots are distinct where the batch is written."""
+class _BatchArrays(NamedTuple):
     slots: torch.Tensor
     starts: torch.Tensor
     lens: torch.Tensor
@@ -209,10 +223,20 @@ class Batch(NamedTuple):
     max_len: int
 
 
+class Batch(_BatchArrays):
+    """The sequences of a call, int32 on the device: sequence b owns rows ``starts[b] .. starts[b + 1] - 1`` of the row tensors and has
+    ``lens[b]`` positions in slot ``slots[b]`` of the cache once they are written, the rows being the last ones.  A slot of -1 is padding.
+    ``max_new`` / ``max_len``: the most new rows / positions of any sequence; they size the launch (results do not depend on them).  The
+    arrays may change between replays of a captured graph.  Slots are distinct where the batch is written."""
+
+
 def _cache(cache: KV8Cache) -> Kv8C:
+    c = cache.__dict__.get("_c")                 # checked and laid out at the object's first use
+    if c is not None:
+        return c
     k, ks, v, vs = cache
     shape = k.shape
-    if k.dim() != 4 or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
+    if len(shape) != 4 or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
         raise ValueError(f"cache: codes [slots, heads, ctx, dim] and scales [slots, heads, ctx] expected, got {list(k.shape)}, {list(ks.shape)}, "
                          f"{list(v.shape)}, {list(vs.shape)}")
     if k.dtype != torch.int8 or v.dtype != torch.int8 or ks.dtype != torch.float32 or vs.dtype != torch.float32:
@@ -221,53 +245,68 @@ def _cache(cache: KV8Cache) -> Kv8C:
         raise ValueError("cache: the four tensors must be on one GPU")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache: contiguous tensors expected")
-    return Kv8C(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), *shape)
+    c = cache.__dict__["_c"] = Kv8C(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), *shape)
+    return c
 
 
-def _batch(batch: Batch, rows: int, device: torch.device) -> Kv8BatchC:
+def _batch(batch: Batch, rows: int, index: int) -> Kv8BatchC:
+    known = batch.__dict__.get("_c")
+    if known is not None and known[0] == rows and known[1] == index:
+        return known[2]
     slots, starts, lens, max_new, max_len = batch
     n = slots.shape[0] if slots.dim() == 1 else -1
     for t, what, want in ((slots, "slots", n), (starts, "starts", n + 1), (lens, "lens", n)):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != want or t.device != device or not t.is_contiguous():
-            raise ValueError(f"batch.{what}: contiguous int32 [{want if want >= 0 else 'seqs'}] on {device} expected, got {t.dtype} {list(t.shape)} on {t.device}")
-    return Kv8BatchC(slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), n, rows, max_new, max_len)
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != want or t.get_device() != index or not t.is_contiguous():
+            raise ValueError(f"batch.{what}: contiguous int32 [{want if want >= 0 else 'seqs'}] on cuda:{index} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+    b = Kv8BatchC(slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), n, rows, max_new, max_len)
+    batch.__dict__["_c"] = (rows, index, b)
+    return b
 
 
-def _head_rows(t: torch.Tensor, what: str, cache: Kv8C, device: torch.device, heads: Optional[int] = None) -> int:
+def _head_rows(t: torch.Tensor, what: str, cache: Kv8C, index: int, heads: Optional[int] = None) -> int:
     """Check ``[rows, heads, dim]`` whose rows may be strided and whose heads lie one after the other; its type code."""
-    if t.dim() != 3 or t.shape[2] != cache.dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what}: [rows, {heads if heads is not None else 'heads'}, {cache.dim}] expected, got {list(t.shape)}")
-    if t.dtype not in _TYPE:
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != cache.dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what}: [rows, {heads if heads is not None else 'heads'}, {cache.dim}] expected, got {list(shape)}")
+    code = _TYPE.get(t.dtype)
+    if code is None:
         raise ValueError(f"{what}: float32, float16 or bfloat16 expected, got {t.dtype}")
-    _place(t, what, device)
-    if t.shape[1] > 1 and t.stride(1) != cache.dim:
-        raise ValueError(f"{what}: the heads of a row must lie one after the other (stride {t.stride(1)})")
-    return _TYPE[t.dtype]
+    if t.get_device() != index:
+        raise ValueError(f"{what}: on {t.device}, expected cuda:{index}")
+    stride = t.stride()
+    if stride[2] != 1 or (shape[1] > 1 and stride[1] != cache.dim):
+        raise ValueError(f"{what}: the heads of a row must lie one after the other, their elements too (strides {stride})")
+    return code
 
 
 def kv_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, batch: Batch) -> None:
     """Quantise the rows ``k`` and ``v`` ``[rows, heads, dim]`` (they may be views of one projection's output) into the cache."""
-    c, device = _cache(cache), cache.k.device
-    dt = _head_rows(k, "k", c, device, c.heads)
-    if _head_rows(v, "v", c, device, c.heads) != dt or v.shape[0] != k.shape[0]:
+    c, index = _cache(cache), cache.k.get_device()
+    dt = _head_rows(k, "k", c, index, c.heads)
+    if _head_rows(v, "v", c, index, c.heads) != dt or v.shape[0] != k.shape[0]:
         raise ValueError(f"v: {list(k.shape)} in {k.dtype} expected, got {list(v.shape)} in {v.dtype}")
-    b = _batch(batch, k.shape[0], device)
-    lib, ctx, stream = _launch(device)
-    _done(lib.wj_kv8_write(ctx, C.byref(c), C.byref(b), dt, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), stream), "wj_kv8_write")
+    b = _batch(batch, k.shape[0], index)
+    lib, ctx, stream = _launch(index)
+    rc = lib.wj_kv8_write(ctx, C.byref(c), C.byref(b), dt, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), stream)
+    if rc:
+        _fail("wj_kv8_write", rc)
 
 
 def kv_read(cache: KV8Cache, batch: Batch, rows: int, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values ``[rows, heads, dim]`` of the batch's rows as the cache holds them (rows behind ``starts[-1]`` are not written)."""
-    c, device = _cache(cache), cache.k.device
+    c, index = _cache(cache), cache.k.get_device()
     if dtype not in _TYPE:
         raise ValueError(f"dtype: float32, float16 or bfloat16 expected, got {dtype}")
     if rows < 0:
         raise ValueError(f"rows: {rows}")
-    b = _batch(batch, rows, device)
-    k = torch.empty((rows, c.heads, c.dim), dtype=dtype, device=device)
-    v = torch.empty_like(k)
-    lib, ctx, stream = _launch(device)
-    _done(lib.wj_kv8_read(ctx, C.byref(c), C.byref(b), _TYPE[dtype], k.data_ptr(), c.heads * c.dim, v.data_ptr(), c.heads * c.dim, stream), "wj_kv8_read")
+    b = _batch(batch, rows, index)
+    heads, dim, device = c.heads, c.dim, cache.k.device
+    k = torch.empty((rows, heads, dim), dtype=dtype, device=device)
+    v = torch.empty((rows, heads, dim), dtype=dtype, device=device)
+    lib, ctx, stream = _launch(index)
+    rc = lib.wj_kv8_read(ctx, C.byref(c), C.byref(b), _TYPE[dtype], k.data_ptr(), heads * dim, v.data_ptr(), heads * dim, stream)
+    if rc:
+        _fail("wj_kv8_read", rc)
     return k, v
 
 
@@ -276,18 +315,20 @@ def kv_attention(q: torch.Tensor, cache: KV8Cache, batch: Batch, *, causal: bool
     """Attention of the rows ``q`` ``[rows, n_heads, dim]`` over the cached positions of their sequences: up to the row's own position
     (``causal``), or all ``lens[b]`` of them.  ``scale`` defaults to ``dim ** -0.5``.  A row that sees nothing is zeros; rows behind
     ``starts[-1]`` are not written."""
-    c, device = _cache(cache), cache.k.device
-    dt = _head_rows(q, "q", c, device)
+    c, index = _cache(cache), cache.k.get_device()
+    dt = _head_rows(q, "q", c, index)
     rows, heads, dim = q.shape
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=device)
-    elif _head_rows(out, "out", c, device, heads) != dt or out.shape[0] != rows or (rows > 1 and out.stride(0) < heads * dim):
+        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
+    elif _head_rows(out, "out", c, index, heads) != dt or out.shape[0] != rows or (rows > 1 and out.stride(0) < heads * dim):
         raise ValueError(f"out: {list(q.shape)} in {q.dtype} expected, rows apart, got {list(out.shape)} in {out.dtype}")
-    b = _batch(batch, rows, device)
-    lib, ctx, stream = _launch(device)
-    need = lib.wj_kv8_attention_workspace(ctx, C.byref(c), C.byref(b), heads)
-    work = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-    _done(lib.wj_kv8_attention(ctx, C.byref(c), C.byref(b), dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), heads,
-                               dim ** -0.5 if scale is None else scale, 1 if causal else 0, work.data_ptr() if work is not None else None, need, stream),
-          "wj_kv8_attention")
+    b = _batch(batch, rows, index)
+    lib, ctx, stream = _launch(index)
+    cp, bp = C.byref(c), C.byref(b)
+    need = lib.wj_kv8_attention_workspace(ctx, cp, bp, heads)
+    work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None      # freed in stream order by torch's allocator
+    rc = lib.wj_kv8_attention(ctx, cp, bp, dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), heads, dim ** -0.5 if scale is None else scale,
+                              1 if causal else 0, work.data_ptr() if need else None, need, stream)
+    if rc:
+        _fail("wj_kv8_attention", rc)
     return out
