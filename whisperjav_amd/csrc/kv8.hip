@@ -27,42 +27,62 @@ __device__ __forceinline__ Span span_of(const Kv8Args& a, int b) {
   return s;
 }
 
-// One wave per (row, head, K or V): the maximum over the lanes, then the codes.
-__global__ __launch_bounds__(256) void kv8_write_kernel(const Kv8Args a, int dtype, const void* __restrict__ k, int64_t ldk,
-                                                        const void* __restrict__ v, int64_t ldv) {
+// Writing: HD / 8 lanes hold one head's row of K and of V, 8 elements each, read and written with one wide access per lane and tensor; the
+// maximum goes over the lanes by exchanges.  Bound by memory: a 16-bit row of 128 moves 256 + 128 + 4 bytes.  A workgroup takes (row, head)
+// pairs of one sequence in turn.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void kv8_write_kernel(const Kv8Args a, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v,
+                                                        int64_t ldv) {
+  constexpr int L = HD / 8, PER = 256 / L;
   const Span s = span_of(a, blockIdx.y);
   if (s.slot < 0) return;
-  const int lane = threadIdx.x & 63, dim = a.c.dim, per = 2 * a.c.heads;
-  const int64_t tasks = (int64_t)s.n * per;
-  for (int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); task < tasks; task += (int64_t)gridDim.x * 4) {
-    const int t = (int)(task / per), which = (int)(task - (int64_t)t * per), head = which >> 1, pos = s.pos0 + t;
-    if (pos < 0 || pos >= a.c.ctx) continue;
-    const bool is_v = which & 1;
-    const void* src = is_v ? v : k;
-    const int64_t at = (int64_t)(s.first + t) * (is_v ? ldv : ldk) + head * dim;
-    const int64_t row = ((int64_t)s.slot * a.c.heads + head) * a.c.ctx + pos;
-    const float x0 = ld_any(src, dtype, at + lane), x1 = dim == 128 ? ld_any(src, dtype, at + 64 + lane) : 0.f;
-    const RowQuant q(wave_max(fmaxf(mag(x0), mag(x1))));
-    int8_t* codes = (is_v ? a.c.v_dev : a.c.k_dev) + row * dim;
-    codes[lane] = (int8_t)q.code(x0);
-    if (dim == 128) codes[64 + lane] = (int8_t)q.code(x1);
-    if (lane == 0) (is_v ? a.c.v_scale_dev : a.c.k_scale_dev)[row] = q.scale;
+  const int l8 = (threadIdx.x % L) * 8, heads = a.c.heads;
+  const int64_t tasks = (int64_t)s.n * heads;
+  for (int64_t task = (int64_t)blockIdx.x * PER + threadIdx.x / L; task < tasks; task += (int64_t)gridDim.x * PER) {
+    const int t = (int)(task / heads), head = (int)(task - (int64_t)t * heads), pos = s.pos0 + t;
+    if (pos < 0 || pos >= a.c.ctx) continue;                    // all lanes of a row alike
+    const Raw8<T> rk = ld_raw8(k + (int64_t)(s.first + t) * ldk + head * HD + l8), rv = ld_raw8(v + (int64_t)(s.first + t) * ldv + head * HD + l8);
+    float xk[8], xv[8], tk = 0.f, tv = 0.f;
+    widen8(rk, xk); widen8(rv, xv);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { tk = fmaxf(tk, mag(xk[e])); tv = fmaxf(tv, mag(xv[e])); }
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) { tk = fmaxf(tk, __shfl_xor(tk, o, 64)); tv = fmaxf(tv, __shfl_xor(tv, o, 64)); }
+    const RowQuant qk(tk), qv(tv);
+    const int64_t row = ((int64_t)s.slot * heads + head) * a.c.ctx + pos;
+    *reinterpret_cast<uint2*>(a.c.k_dev + row * HD + l8) = make_uint2(pack4(qk.code(xk[0]), qk.code(xk[1]), qk.code(xk[2]), qk.code(xk[3])),
+                                                                      pack4(qk.code(xk[4]), qk.code(xk[5]), qk.code(xk[6]), qk.code(xk[7])));
+    *reinterpret_cast<uint2*>(a.c.v_dev + row * HD + l8) = make_uint2(pack4(qv.code(xv[0]), qv.code(xv[1]), qv.code(xv[2]), qv.code(xv[3])),
+                                                                      pack4(qv.code(xv[4]), qv.code(xv[5]), qv.code(xv[6]), qv.code(xv[7])));
+    if (l8 == 0) { a.c.k_scale_dev[row] = qk.scale; a.c.v_scale_dev[row] = qv.scale; }
   }
 }
 
-__global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, int dtype, void* __restrict__ k, int64_t ldk, void* __restrict__ v,
-                                                       int64_t ldv) {
+__device__ __forceinline__ void codes8(uint2 w, float s, float v[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = (float)(int8_t)(w.x >> (8 * e)) * s;
+    v[4 + e] = (float)(int8_t)(w.y >> (8 * e)) * s;
+  }
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, T* __restrict__ k, int64_t ldk, T* __restrict__ v, int64_t ldv) {
+  constexpr int L = HD / 8, PER = 256 / L;
   const Span s = span_of(a, blockIdx.y);
-  const int lane = threadIdx.x & 63, dim = a.c.dim, per = 2 * a.c.heads;
-  const int64_t tasks = (int64_t)s.n * per;
-  for (int64_t task = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); task < tasks; task += (int64_t)gridDim.x * 4) {
-    const int t = (int)(task / per), which = (int)(task - (int64_t)t * per), head = which >> 1, pos = s.pos0 + t;
-    const bool is_v = which & 1, there = s.slot >= 0 && pos >= 0 && pos < a.c.ctx;
-    const int64_t at = (int64_t)(s.first + t) * (is_v ? ldv : ldk) + head * dim;
-    const int64_t row = there ? ((int64_t)s.slot * a.c.heads + head) * a.c.ctx + pos : 0;
-    const int8_t* codes = (is_v ? a.c.v_dev : a.c.k_dev) + row * dim;
-    const float scale = (is_v ? a.c.v_scale_dev : a.c.k_scale_dev)[row];
-    for (int d = lane; d < dim; d += 64) st_any(is_v ? v : k, dtype, at + d, there ? (float)codes[d] * scale : 0.f);
+  const int l8 = (threadIdx.x % L) * 8, heads = a.c.heads;
+  const int64_t tasks = (int64_t)s.n * heads;
+  for (int64_t task = (int64_t)blockIdx.x * PER + threadIdx.x / L; task < tasks; task += (int64_t)gridDim.x * PER) {
+    const int t = (int)(task / heads), head = (int)(task - (int64_t)t * heads), pos = s.pos0 + t;
+    float xk[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, xv[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (s.slot >= 0 && pos >= 0 && pos < a.c.ctx) {
+      const int64_t row = ((int64_t)s.slot * heads + head) * a.c.ctx + pos;
+      const uint2 wk = *reinterpret_cast<const uint2*>(a.c.k_dev + row * HD + l8), wv = *reinterpret_cast<const uint2*>(a.c.v_dev + row * HD + l8);
+      codes8(wk, a.c.k_scale_dev[row], xk);
+      codes8(wv, a.c.v_scale_dev[row], xv);
+    }
+    st8<T>(k + (int64_t)(s.first + t) * ldk + head * HD + l8, xk);
+    st8<T>(v + (int64_t)(s.first + t) * ldv + head * HD + l8, xv);
   }
 }
 
@@ -420,6 +440,44 @@ int check_kv8(const char* who, wj_ctx* ctx, const wj_kv8* c, const wj_kv8_batch*
   return WJ_OK;
 }
 
+// (row, head) pairs of a sequence over workgroups: at most 4 turns each while there are enough of them
+dim3 pair_grid(int64_t pairs, int per, int seqs) {
+  const int64_t groups = (pairs + per - 1) / per, want = groups * seqs > 8192 ? (groups + 3) / 4 : groups;
+  return dim3((unsigned)(want < 65536 ? want : 65536), seqs);
+}
+template <typename T, int HD>
+int start_write(const wj_kv8* c, const wj_kv8_batch* b, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t pairs, hipStream_t s) {
+  hipLaunchKernelGGL((kv8_write_kernel<T, HD>), pair_grid(pairs, 256 / (HD / 8), b->seqs), dim3(256), 0, s, Kv8Args{*c, *b}, (const T*)k, ldk, (const T*)v, ldv);
+  WJ_LAUNCH_CHECK();
+  return WJ_OK;
+}
+template <typename T, int HD>
+int start_read(const wj_kv8* c, const wj_kv8_batch* b, void* k, int64_t ldk, void* v, int64_t ldv, int64_t pairs, hipStream_t s) {
+  hipLaunchKernelGGL((kv8_read_kernel<T, HD>), pair_grid(pairs, 256 / (HD / 8), b->seqs), dim3(256), 0, s, Kv8Args{*c, *b}, (T*)k, ldk, (T*)v, ldv);
+  WJ_LAUNCH_CHECK();
+  return WJ_OK;
+}
+int launch_write(const wj_kv8* c, const wj_kv8_batch* b, int dtype, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t pairs, hipStream_t s) {
+  if (c->dim == 128) {
+    if (dtype == WJ_F32) return start_write<float, 128>(c, b, k, ldk, v, ldv, pairs, s);
+    if (dtype == WJ_F16) return start_write<f16_t, 128>(c, b, k, ldk, v, ldv, pairs, s);
+    return start_write<bf16_t, 128>(c, b, k, ldk, v, ldv, pairs, s);
+  }
+  if (dtype == WJ_F32) return start_write<float, 64>(c, b, k, ldk, v, ldv, pairs, s);
+  if (dtype == WJ_F16) return start_write<f16_t, 64>(c, b, k, ldk, v, ldv, pairs, s);
+  return start_write<bf16_t, 64>(c, b, k, ldk, v, ldv, pairs, s);
+}
+int launch_read(const wj_kv8* c, const wj_kv8_batch* b, int dtype, void* k, int64_t ldk, void* v, int64_t ldv, int64_t pairs, hipStream_t s) {
+  if (c->dim == 128) {
+    if (dtype == WJ_F32) return start_read<float, 128>(c, b, k, ldk, v, ldv, pairs, s);
+    if (dtype == WJ_F16) return start_read<f16_t, 128>(c, b, k, ldk, v, ldv, pairs, s);
+    return start_read<bf16_t, 128>(c, b, k, ldk, v, ldv, pairs, s);
+  }
+  if (dtype == WJ_F32) return start_read<float, 64>(c, b, k, ldk, v, ldv, pairs, s);
+  if (dtype == WJ_F16) return start_read<f16_t, 64>(c, b, k, ldk, v, ldv, pairs, s);
+  return start_read<bf16_t, 64>(c, b, k, ldk, v, ldv, pairs, s);
+}
+
 // Rows per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).
 struct AttnPlan { int rt, nsplit, chunk; };
 AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
@@ -473,11 +531,8 @@ int wj_kv8_write(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, in
   WJ_REQUIRE(ldk >= 0 && ldv >= 0, "wj_kv8_write: negative stride");
   DeviceScope dev;
   WJ_HIP(dev.enter(ctx->device));
-  const int64_t tasks = (int64_t)(batch->max_new > 0 ? batch->max_new : 1) * 2 * cache->heads;
-  const unsigned gx = (unsigned)(tasks + 3 < 4 * 4096 ? (tasks + 3) / 4 : 4096);
-  hipLaunchKernelGGL(kv8_write_kernel, dim3(gx, batch->seqs), dim3(256), 0, ctx->pick(stream), Kv8Args{*cache, *batch}, dtype, k_dev, ldk, v_dev, ldv);
-  WJ_LAUNCH_CHECK();
-  return WJ_OK;
+  const int64_t pairs = (int64_t)(batch->max_new > 0 ? batch->max_new : 1) * cache->heads;
+  return launch_write(cache, batch, dtype, k_dev, ldk, v_dev, ldv, pairs, ctx->pick(stream));
 }
 
 int wj_kv8_read(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int dtype, void* k_dev, int64_t ldk, void* v_dev, int64_t ldv,
@@ -489,11 +544,8 @@ int wj_kv8_read(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int
   WJ_REQUIRE(batch->rows == 1 || (ldk >= cache->heads * cache->dim && ldv >= cache->heads * cache->dim), "wj_kv8_read: output rows overlap");
   DeviceScope dev;
   WJ_HIP(dev.enter(ctx->device));
-  const int64_t tasks = (int64_t)(batch->max_new > 0 ? batch->max_new : 1) * 2 * cache->heads;
-  const unsigned gx = (unsigned)(tasks + 3 < 4 * 4096 ? (tasks + 3) / 4 : 4096);
-  hipLaunchKernelGGL(kv8_read_kernel, dim3(gx, batch->seqs), dim3(256), 0, ctx->pick(stream), Kv8Args{*cache, *batch}, dtype, k_dev, ldk, v_dev, ldv);
-  WJ_LAUNCH_CHECK();
-  return WJ_OK;
+  const int64_t pairs = (int64_t)(batch->max_new > 0 ? batch->max_new : 1) * cache->heads;
+  return launch_read(cache, batch, dtype, k_dev, ldk, v_dev, ldv, pairs, ctx->pick(stream));
 }
 
 int64_t wj_kv8_attention_workspace(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int n_heads) {
