@@ -325,6 +325,33 @@ def test_attention(q8, layout, dim, heads, per, dtype, causal):
         assert bool((out[:, heads * per] == 0).all()) and bool((out[-1] == 0).all())
 
 
+@pytest.mark.parametrize("dim,heads,per", [(64, 4, 1), (64, 2, 3), (128, 3, 2), (128, 2, 4)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_of_many_prompts(q8, dim, heads, per, dtype, causal):
+    """whole prompts and later parts of them, enough of them for the kernel that takes 128 rows at a time"""
+    g, ctx, n_slots = rng(dim * heads + per), 210, 30
+    slots = torch.randperm(n_slots, generator=g).tolist()[:26]
+    slots[3], slots[9] = -1, n_slots
+    starts, lens = [0], []
+    for b in range(26):
+        n = int(torch.randint(0, 60, (1,), generator=g)) * (3 if b % 4 == 0 else 1)
+        starts.append(starts[-1] + n)
+        lens.append(n if b % 3 else min(ctx, n + 37))
+    lens[5], lens[6] = max(0, lens[5] - 7), 64                              # rows before position 0; whole 64s
+    host, values = filled_cache(q8, g, n_slots, heads, ctx, dim)
+    poison_behind(host, slots, lens, causal)
+    cache = q8.KV8Cache(*(t.cuda() for t in host))
+    rows = starts[-1] + 3
+    q = (torch.randn(rows, heads * per, dim, generator=g) * 1.5).to(dtype)
+    out = torch.zeros(rows, heads * per + 1, dim, dtype=dtype).cuda()
+    for hint in (None, 150):
+        batch = make_batch(q8, slots, starts, lens, hint)
+        got = q8.kv_attention(q.cuda(), cache, batch, causal=causal, out=out[:, : heads * per])
+        check_attention(got, q, values, slots, starts, lens, causal, dim ** -0.5, dtype)
+        assert bool((out[:, heads * per] == 0).all()) and bool((out[starts[-1]:] == 0).all())
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("new,length", [(1, 5000), (3, 4099), (20, 3001), (70, 2500)])
 def test_attention_over_a_long_cache(q8, dtype, new, length):

@@ -15,13 +15,15 @@ struct Kv8Args {
 // What a sequence of the call owns.  first .. first + n - 1: its rows of the row arrays; pos0: position of the first of them
 struct Span { int slot, first, n, len, pos0; };
 __device__ __forceinline__ Span span_of(const Kv8Args& a, int b) {
+  // the same for every lane: kept in scalar registers
+  auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
   Span s;
-  s.slot = a.b.slots_dev[b];
-  s.first = a.b.starts_dev[b];
-  const int last = min(a.b.starts_dev[b + 1], a.b.rows);
+  s.slot = uni(a.b.slots_dev[b]);
+  s.first = uni(a.b.starts_dev[b]);
+  const int last = min(uni(a.b.starts_dev[b + 1]), a.b.rows);
   if (s.first < 0) s.first = a.b.rows;                 // not a span of the arrays: no rows
   s.n = max(0, last - s.first);
-  s.len = a.b.lens_dev[b];
+  s.len = uni(a.b.lens_dev[b]);
   s.pos0 = s.len - s.n;
   if (s.slot < 0 || s.slot >= a.c.slots) s.slot = -1;
   return s;
@@ -405,6 +407,190 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
   }
 }
 
+// Many rows: 128 rows of one key / value head per workgroup, 32 per wave, positions 64 at a time through LDS.  The codes are widened to
+// halves ONCE per workgroup on their way into LDS (both operands in the order the products read them: K rows permuted, V transposed in
+// registers, 8 positions of one dimension per 16-byte piece), which the rows kernel above does once per wave.  The next 64 positions are
+// in flight (registers) while this wave's products run.  Two buffers, one barrier per step, two workgroups per CU.
+template <typename T, int HD>
+__global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a, int blocks) {
+  constexpr int NP = sizeof(T) == 4 ? 2 : 1;
+  constexpr int NW = std::is_same<T, bf16_t>::value ? 1 : 2;
+  constexpr int NE = HD / 16, KS = HD / 32;
+  constexpr int KB = 64 * HD * 2, VB = 64 * HD * 2, BUF = KB + VB + 3 * 256;       // K [64][HD], V^T [HD][64], then ks, vs, exponents [64]
+  constexpr int KL = HD / 64;                                                      // 16-byte pieces of K per thread
+  extern __shared__ __attribute__((aligned(16))) char lds_t[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
+  // workgroups go to the 8 XCDs in turn: all row blocks of one (sequence, head) on one XCD, the longest first
+  const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3, group = idx / blocks * 8 + xcd;
+  if (group >= a.s.b.seqs * a.s.c.heads) return;
+  const int seq = group / a.s.c.heads, kvh = group - seq * a.s.c.heads;
+  const Span s = span_of(a.s, seq);
+  const int rows = s.n * a.per, n_blocks = (rows + 127) >> 7;
+  const int64_t row0 = ((int64_t)max(s.slot, 0) * a.s.c.heads + kvh) * a.s.c.ctx;
+  const int8_t* kp = a.s.c.k_dev + row0 * HD;
+  const int8_t* vp = a.s.c.v_dev + row0 * HD;
+  const float* ksp = a.s.c.k_scale_dev + row0;
+  const float* vsp = a.s.c.v_scale_dev + row0;
+  for (int block = n_blocks - 1 - idx % blocks; block >= 0; block -= blocks) {
+    const int first = block * 128, last = min(rows, first + 128) - 1;
+    const int wfirst = first + wave * 32, wlast = min(last, wfirst + 31);
+    const int kend = row_limit(a, s, last);                                        // positions the workgroup walks
+    const int wend = wfirst <= last ? row_limit(a, s, wlast) : 0, every = wfirst <= last ? row_limit(a, s, wfirst) : 0;
+
+    f16x8_t qf[2][NP][KS];
+    float unit[2], M[2], l[2];
+    int limit[2];
+    f32x4_t o[2][NE];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int r = wfirst + t * 16 + li;
+      unit[t] = load_query<T, HD, NP>(a, s, kvh, r, rows, lg, qf[t]);
+      limit[t] = r <= last ? row_limit(a, s, r) : kend;
+      M[t] = -INFINITY; l[t] = 0.f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // this thread's share of 64 positions: KL pieces of K; 8 positions x 4 dimensions of V (HD = 64: half of the threads); one scale
+    uint4 rk[KL];
+    uint32_t rv[8];
+    float rs = 0.f;
+    const int vd = tid % (HD / 4), vg = tid / (HD / 4);                            // V: dimensions 4 vd .., positions 8 vg ..
+    auto fetch = [&](int kt) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        const int u = i * 256 + tid, key = min(kt + u / (HD / 16), kend - 1);
+        rk[i] = *reinterpret_cast<const uint4*>(kp + (int64_t)key * HD + (u % (HD / 16)) * 16);
+      }
+      if (HD == 128 || vg < 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rv[j] = *reinterpret_cast<const uint32_t*>(vp + (int64_t)min(kt + vg * 8 + j, kend - 1) * HD + vd * 4);
+      }
+      if (tid < 128) rs = (tid < 64 ? ksp : vsp)[min(kt + (tid & 63), kend - 1)];
+    };
+    auto put = [&](int buf) __attribute__((always_inline)) {
+      char* b = lds_t + buf * BUF;
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        const int u = i * 256 + tid, key = u / (HD / 16), c = (u % (HD / 16)) * 2;
+        // the row this position has in the first product's operand
+        const int row = (key >> 5) * 32 + ((key >> 2) & 1) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
+        const int x = row & (HD / 8 - 1);
+        *reinterpret_cast<f16x8_t*>(b + row * (HD * 2) + ((c ^ x) << 4)) = codes_to_h8(rk[i].x, rk[i].y);
+        *reinterpret_cast<f16x8_t*>(b + row * (HD * 2) + (((c + 1) ^ x) << 4)) = codes_to_h8(rk[i].z, rk[i].w);
+      }
+      if (HD == 128 || vg < 8) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = rv[j] ^ 0x80808080u;
+        char* v = b + KB + vd * 4 * 128 + ((vg ^ (vd & 7)) << 4);
+        *reinterpret_cast<uint4*>(v) = make_uint4(codes_pair<0>(w[0], w[1]), codes_pair<0>(w[2], w[3]), codes_pair<0>(w[4], w[5]), codes_pair<0>(w[6], w[7]));
+        *reinterpret_cast<uint4*>(v + 128) = make_uint4(codes_pair<1>(w[0], w[1]), codes_pair<1>(w[2], w[3]), codes_pair<1>(w[4], w[5]), codes_pair<1>(w[6], w[7]));
+        *reinterpret_cast<uint4*>(v + 256) = make_uint4(codes_pair<2>(w[0], w[1]), codes_pair<2>(w[2], w[3]), codes_pair<2>(w[4], w[5]), codes_pair<2>(w[6], w[7]));
+        *reinterpret_cast<uint4*>(v + 384) = make_uint4(codes_pair<3>(w[0], w[1]), codes_pair<3>(w[2], w[3]), codes_pair<3>(w[4], w[5]), codes_pair<3>(w[6], w[7]));
+      }
+      float* sc = reinterpret_cast<float*>(b + KB + VB);
+      if (tid < 128) sc[tid] = rs;
+      if (tid >= 64 && tid < 128) sc[64 + tid] = scale_exponent(rs);
+    };
+
+    // 32 positions: half h of the buffer's 64
+    auto tile = [&](const int kt, const int buf, const int h, auto masked_tag) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      const char* b = lds_t + buf * BUF;
+      const float* sc = reinterpret_cast<const float*>(b + KB + VB) + h * 32 + lg * 8;
+      const int key0 = kt + h * 32 + lg * 8;
+      f32x4_t st[2][2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        st[0][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        st[1][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        const int row = h * 32 + kb * 16 + li;
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+          const f16x8_t kf = *reinterpret_cast<const f16x8_t*>(b + row * (HD * 2) + (((lg * KS + c) ^ (li & (HD / 8 - 1))) << 4));
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) st[t][kb] = mfma16(kf, qf[t][p][c], st[t][kb]);
+        }
+      }
+      f16x8_t pf[2][NW];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float x[8], top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = st[t][j >> 2][j & 3] * sc[j] * unit[t];
+          const bool in = !MASKED || key0 + j < limit[t];
+          top = fmaxf(top, in ? x[j] + sc[128 + j] : -INFINITY);
+        }
+        top = quad_max(top);
+        if (top > M[t] + kSlack) {
+          const float f = __builtin_amdgcn_exp2f(M[t] - top);
+          M[t] = top;
+          l[t] *= f;
+#pragma unroll
+          for (int e = 0; e < NE; ++e)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][e][r] *= f;
+        }
+        const float m = M[t] == -INFINITY ? 0.f : M[t];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool in = !MASKED || key0 + j < limit[t];
+          const float p = in ? __builtin_amdgcn_exp2f(x[j] - m) : 0.f;
+          l[t] += p;
+          const float w = in ? p * sc[64 + j] : 0.f;
+          const f16_t hi = f2h(w);
+          pf[t][0][j] = hi;
+          if constexpr (NW == 2) pf[t][1][j] = f2h(w - h2f(hi));
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const int d = e * 16 + li;
+        const f16x8_t vf = *reinterpret_cast<const f16x8_t*>(b + KB + d * 128 + (((h * 4 + lg) ^ ((d >> 2) & 7)) << 4));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int p = 0; p < NW; ++p) o[t][e] = mfma16(vf, pf[t][p], o[t][e]);
+      }
+    };
+
+    __syncthreads();                       // the block before has read its last buffer
+    if (kend > 0) { fetch(0); put(0); }
+    __syncthreads();
+    int buf = 0;
+    for (int kt = 0; kt < kend; kt += 64, buf ^= 1) {
+      const bool more = kt + 64 < kend;
+      if (more) fetch(kt + 64);
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        if (kt + h * 32 + 32 <= every) tile(kt, buf, h, std::false_type{});
+        else if (kt + h * 32 < wend) tile(kt, buf, h, std::true_type{});
+      }
+      if (more) put(buf ^ 1);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float sum = quad_sum(l[t]);
+      const int r = wfirst + t * 16 + li;
+      if (r > last) continue;
+      const float inv = limit[t] > 0 ? 1.f / sum : 0.f;
+      T* out = reinterpret_cast<T*>(a.out) + (int64_t)(s.first + r / a.per) * a.ldo + (kvh * a.per + r % a.per) * HD + lg * 4;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = limit[t] > 0 ? o[t][e][i] * inv : 0.f;
+        st_out<T, 4>(out + e * 16, v);
+      }
+    }
+  }
+}
+
 // The parts of every row's positions joined, in order: 16 lanes per (row, head)
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const AttnArgs a, int block_rows) {
@@ -479,11 +665,12 @@ int launch_read(const wj_kv8* c, const wj_kv8_batch* b, int dtype, void* k, int6
 }
 
 // Rows per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).
-struct AttnPlan { int rt, nsplit, chunk; };
+struct AttnPlan { int rt, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel
 AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
   const int per = n_heads / c.heads;
   const int64_t rows = (int64_t)(b.max_new > 0 ? b.max_new : 1) * per;
   AttnPlan p;
+  if (rows > 64 && (int64_t)b.seqs * c.heads * ((rows + 127) / 128) >= 128) return {0, 1, 0};
   p.rt = rows <= 16 ? 1 : 2;
   const int64_t groups = (int64_t)b.seqs * c.heads * ((rows + 16 * p.rt - 1) / (16 * p.rt));
   const int len = b.max_len < c.ctx ? (b.max_len > 0 ? b.max_len : 1) : c.ctx;
@@ -508,8 +695,22 @@ int start_attention(const AttnArgs& a, hipStream_t s) {
   }
   return WJ_OK;
 }
+template <typename T, int HD>
+int start_tile(const AttnArgs& a, hipStream_t s) {
+  static AttrOnce once;
+  constexpr int lds = 2 * (64 * HD * 4 + 768);
+  if (once.need()) {
+    WJ_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kv8_attn_tile_kernel<T, HD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    once.done();
+  }
+  const int64_t rows = (int64_t)a.s.b.max_new * a.per, blocks = (rows + 127) / 128, groups = (int64_t)a.s.b.seqs * a.s.c.heads;
+  hipLaunchKernelGGL((kv8_attn_tile_kernel<T, HD>), dim3((unsigned)((groups + 7) / 8 * 8 * blocks)), dim3(256), lds, s, a, (int)blocks);
+  WJ_LAUNCH_CHECK();
+  return WJ_OK;
+}
 template <int HD, typename T>
 int pick_rows(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+  if (p.rt == 0) return start_tile<T, HD>(a, s);
   return p.rt == 1 ? start_attention<T, HD, 1>(a, s) : start_attention<T, HD, 2>(a, s);
 }
 template <int HD>
