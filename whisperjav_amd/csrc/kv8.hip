@@ -110,8 +110,8 @@ struct AttnArgs {
   const void* q; int64_t ldq;
   void* out; int64_t ldo;
   int n_heads, per, causal;
-  float scale2;              // |scale| * log2(e)
-  float sign;                // of scale, goes onto the query
+  uint32_t per_inv;          // ceil(2^32 / per): r / per is the high word of r * per_inv for r < 2^28 (per = 1: 0, see over_per)
+  float scale2;              // scale * log2(e)
   int chunk, nsplit;         // positions per workgroup; workgroups per row block (the last takes what is left)
   float* part;               // nsplit > 1: numerator sums [row * n_heads + head][nsplit][dim]
   float2* ml;                // ... and (M, denominator)
@@ -156,40 +156,69 @@ __device__ __forceinline__ float scale_exponent(float vs) {      // of a value s
   return vs == 0.f ? -100.f : fminf(fmaxf((float)__builtin_amdgcn_frexp_expf(vs), -100.f), 110.f);
 }
 
+__device__ __forceinline__ int over_per(const AttnArgs& a, int r) { return a.per == 1 ? r : (int)__umulhi((uint32_t)r, a.per_inv); }
+
 // the positions that rows r0 .. of a block may see at most, and the row's own
 __device__ __forceinline__ int row_limit(const AttnArgs& a, const Span& s, int r) {
   if (s.slot < 0) return 0;
-  return max(0, min(a.s.c.ctx, a.causal ? s.pos0 + r / a.per + 1 : s.len));
+  return max(0, min(a.s.c.ctx, a.causal ? s.pos0 + over_per(a, r) + 1 : s.len));
 }
 
-// The query fragments of row r (this lane's 8 dims of every 32-dim step, see the kernels' dims), in units of 2^ex of its row: NP halves each
-template <typename T, int HD, int NP>
+// The query operands of row r: piece c holds dims lg * (HD / 4) + 8 c (or, INTERLEAVED, 32 c + 8 lg), NP halves each; returns what a product
+// counts in units of log2.  float16 rows go in as they are.  The others are counted in units of a power of two that bounds the row: a
+// bfloat16 value is then exact in float16 down to 2^-14 of the row's largest, a float32 one is its high and its low half (22 bits).
+// A row that is not finite makes NaN of its own scores.
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+template <typename T, int HD, int NP, bool INTERLEAVED>
 __device__ __forceinline__ float load_query(const AttnArgs& a, const Span& s, int kvh, int r, int rows, int lg, f16x8_t (&qf)[NP][HD / 32]) {
-  float v[HD / 4], top = 0.f;
+  constexpr int KS = HD / 32;
+  Raw8<T> raw[KS];
+#pragma unroll
+  for (int c = 0; c < KS; ++c)
+#pragma unroll
+    for (int w = 0; w < (int)(2 * sizeof(T)); ++w) raw[c].w[w] = 0u;
   if (r < rows) {
-    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(s.first + r / a.per) * a.ldq + (int64_t)(kvh * a.per + r % a.per) * HD + lg * (HD / 4);
+    const int t = over_per(a, r);
+    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(s.first + t) * a.ldq + (kvh * a.per + r - t * a.per) * HD;
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c) widen8(ld_raw8(p + c * 8), v + c * 8);
-  } else {
-#pragma unroll
-    for (int e = 0; e < HD / 4; ++e) v[e] = 0.f;
+    for (int c = 0; c < KS; ++c) raw[c] = ld_raw8(p + (INTERLEAVED ? 32 * c + 8 * lg : lg * (HD / 4) + 8 * c));
   }
+  if constexpr (std::is_same<T, f16_t>::value) {
 #pragma unroll
-  for (int e = 0; e < HD / 4; ++e) top = fmaxf(top, mag(v[e]));
-  top = quad_max(top);
-  // |v| / unit <= 1; a row that is not finite gets a NaN unit, which makes NaN of its scores alone
-  const int ex = top > 0.f ? max(__builtin_amdgcn_frexp_expf(top), -120) : 0;
-  const float down = ldexpf(a.sign, -ex);
+    for (int c = 0; c < KS; ++c) qf[0][c] = __builtin_bit_cast(f16x8_t, raw[c]);
+    return a.scale2;
+  } else {
+    float v[KS][8], top = 0.f;
+    if constexpr (sizeof(T) == 2) {
+      u16x2_t t = {0, 0};
 #pragma unroll
-  for (int c = 0; c < HD / 32; ++c)
+      for (int c = 0; c < KS; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = top < INFINITY ? v[c * 8 + e] * down : 0.f;
-      const f16_t hi = f2h(x);
-      qf[0][c][e] = hi;
-      if constexpr (NP == 2) qf[1][c][e] = f2h(x - h2f(hi));
+        for (int w = 0; w < 4; ++w) t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2_t, raw[c].w[w] & 0x7fff7fffu));
+      top = mag(__uint_as_float((uint32_t)max(t[0], t[1]) << 16));
     }
-  return top < INFINITY ? ldexpf(a.scale2, ex) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int c = 0; c < KS; ++c) {
+      widen8(raw[c], v[c]);
+      if constexpr (sizeof(T) == 4)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, mag(v[c][e]));
+    }
+    top = quad_max(top);
+    const bool fine = top < INFINITY;
+    const int ex = top > 0.f && fine ? max(__builtin_amdgcn_frexp_expf(top), -120) : 0;
+    const float down = fine ? ldexpf(1.f, -ex) : 0.f;
+#pragma unroll
+    for (int c = 0; c < KS; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = v[c][e] * down;
+        const f16_t hi = f2h(x);
+        qf[0][c][e] = hi;
+        if constexpr (NP == 2) qf[1][c][e] = f2h(x - h2f(hi));
+      }
+    return fine ? ldexpf(a.scale2, ex) : __uint_as_float(0x7fc00000u);
+  }
 }
 
 template <typename T, int N> __device__ __forceinline__ void st_out(T* p, const float* v) {      // any alignment: gfx950 serves wide unaligned stores
@@ -218,7 +247,7 @@ template <int N> struct Part {
 };
 
 template <typename T, int HD, int RT>
-__global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv8_attn_rows_kernel(const AttnArgs a) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;                              // halves of a query
   constexpr int NW = std::is_same<T, bf16_t>::value ? 1 : 2;              // halves of a weight
   constexpr int NE = HD / 16;                  // 16-dim tiles of the output; a lane's output dims are NE consecutive ones, four times
@@ -250,7 +279,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int r = first + t * 16 + li;
-      unit[t] = load_query<T, HD, NP>(a, s, kvh, r, (int)rows, lg, qf[t]);
+      unit[t] = load_query<T, HD, NP, false>(a, s, kvh, r, (int)rows, lg, qf[t]);
       limit[t] = r <= last ? min(kend, row_limit(a, s, r)) : kend;
       M[t] = -INFINITY; l[t] = 0.f;
 #pragma unroll
@@ -318,9 +347,9 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
         float x[8], top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          x[j] = st[t][j >> 2][j & 3] * ks[j] * unit[t];
+          x[j] = st[t][j >> 2][j & 3] * ks[j];
           const bool in = !MASKED || kt + 8 * lg + j < limit[t];
-          top = fmaxf(top, in ? x[j] + ex[j] : -INFINITY);
+          top = fmaxf(top, in ? fmaf(x[j], unit[t], ex[j]) : -INFINITY);
         }
         top = quad_max(top);
         if (top > M[t] + kSlack) {
@@ -336,7 +365,7 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool in = !MASKED || kt + 8 * lg + j < limit[t];
-          const float p = in ? __builtin_amdgcn_exp2f(x[j] - m) : 0.f;
+          const float p = in ? __builtin_amdgcn_exp2f(fmaf(x[j], unit[t], -m)) : 0.f;
           l[t] += p;
           const float w = in ? p * vs[j] : 0.f;
           const f16_t hi = f2h(w);
@@ -392,7 +421,8 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
         for (int w = 0; w < 4; ++w) p.see(lml[w * 16 + row]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) p.add(lml[w * 16 + row], &lo[(w * 16 + row) * LDO + d0]);
-        const int64_t at = (int64_t)(s.first + r / a.per), head = kvh * a.per + r % a.per;
+        const int t1 = over_per(a, r);
+        const int64_t at = s.first + t1, head = kvh * a.per + r - t1 * a.per;
         if (a.nsplit == 1) {
           p.finish(row_limit(a, s, r) > 0);
           st_out<T, NE>(reinterpret_cast<T*>(a.out) + at * a.ldo + head * HD + d0, p.o);
@@ -407,14 +437,17 @@ __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(const AttnArgs a) {
   }
 }
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+// `bytes` bytes from p as a buffer: loads past them give zeros
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void* p, int bytes) { return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00027000); }
+
 // Many rows: 128 rows of one key / value head per workgroup, 32 per wave, positions 64 at a time through LDS.  The codes are widened to
 // halves ONCE per workgroup on their way into LDS (both operands in the order the products read them: K rows permuted, V transposed in
 // registers, 8 positions of one dimension per 16-byte piece), which the rows kernel above does once per wave.  The next 64 positions are
 // in flight (registers) while this wave's products run.  Two buffers, one barrier per step, two workgroups per CU.
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a, int blocks) {
-  constexpr int NP = sizeof(T) == 4 ? 2 : 1;
-  constexpr int NW = std::is_same<T, bf16_t>::value ? 1 : 2;
+  constexpr int NP = 1, NW = std::is_same<T, bf16_t>::value ? 1 : 2;
   constexpr int NE = HD / 16, KS = HD / 32;
   constexpr int KB = 64 * HD * 2, VB = 64 * HD * 2, BUF = KB + VB + 3 * 256;       // K [64][HD], V^T [HD][64], then ks, vs, exponents [64]
   constexpr int KL = HD / 64;                                                      // 16-byte pieces of K per thread
@@ -427,16 +460,65 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
   const Span s = span_of(a.s, seq);
   const int rows = s.n * a.per, n_blocks = (rows + 127) >> 7;
   const int64_t row0 = ((int64_t)max(s.slot, 0) * a.s.c.heads + kvh) * a.s.c.ctx;
-  const int8_t* kp = a.s.c.k_dev + row0 * HD;
-  const int8_t* vp = a.s.c.v_dev + row0 * HD;
-  const float* ksp = a.s.c.k_scale_dev + row0;
-  const float* vsp = a.s.c.v_scale_dev + row0;
+  const auto k_buf = buffer_of(a.s.c.k_dev + row0 * HD, a.s.c.ctx * HD), v_buf = buffer_of(a.s.c.v_dev + row0 * HD, a.s.c.ctx * HD);
+  const auto ks_buf = buffer_of(a.s.c.k_scale_dev + row0, a.s.c.ctx * 4), vs_buf = buffer_of(a.s.c.v_scale_dev + row0, a.s.c.ctx * 4);
   for (int block = n_blocks - 1 - idx % blocks; block >= 0; block -= blocks) {
     const int first = block * 128, last = min(rows, first + 128) - 1;
     const int wfirst = first + wave * 32, wlast = min(last, wfirst + 31);
     const int kend = row_limit(a, s, last);                                        // positions the workgroup walks
     const int wend = wfirst <= last ? row_limit(a, s, wlast) : 0, every = wfirst <= last ? row_limit(a, s, wfirst) : 0;
 
+    // this thread's share of 64 positions: KL pieces of K; 8 positions x 4 dimensions of V (HD = 64: half of the threads); one scale.
+    // Positions behind kend are fetched like the others (their weights are cleared); those behind the slot's last one read as zeros, which is
+    // what a buffer load gives past its range.
+    u32x4_t rk[KL];
+    uint32_t rv[8], rs = 0;
+    const int vd = tid % (HD / 4), vg = tid / (HD / 4);                            // V: dimensions 4 vd .., positions 8 vg ..
+    const bool has_v = HD == 128 || vg < 8;
+    auto fetch = [&](int kt) __attribute__((always_inline)) {
+      const int k = kt * HD + tid * 16, v = kt * HD + vg * 8 * HD + vd * 4;        // bytes from the slot's first position
+#pragma unroll
+      for (int i = 0; i < KL; ++i) rk[i] = __builtin_amdgcn_raw_buffer_load_b128(k_buf, k + i * 4096, 0, 0);
+      if (has_v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rv[j] = __builtin_amdgcn_raw_buffer_load_b32(v_buf, v + j * HD, 0, 0);
+      }
+      if (tid < 64) rs = __builtin_amdgcn_raw_buffer_load_b32(ks_buf, (kt + tid) * 4, 0, 0);
+      else if (tid < 128) rs = __builtin_amdgcn_raw_buffer_load_b32(vs_buf, (kt + tid - 64) * 4, 0, 0);
+    };
+    int k_put[KL];                                                                 // the first of a piece's two halves; the second: ^ 16
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      const int u = i * 256 + tid, key = u / (HD / 16), c = (u % (HD / 16)) * 2;
+      // the row this position has in the first product's operand
+      const int row = (key >> 5) * 32 + ((key >> 2) & 1) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
+      k_put[i] = row * (HD * 2) + ((c ^ (row & (HD / 8 - 1))) << 4);
+    }
+    const int v_put[2] = {KB + vd * 512 + ((vg ^ ((2 * vd) & 7)) << 4), KB + vd * 512 + ((vg ^ ((2 * vd + 1) & 7)) << 4)};
+    auto put = [&](int buf) __attribute__((always_inline)) {
+      char* b = lds_t + buf * BUF;
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        *reinterpret_cast<f16x8_t*>(b + k_put[i]) = codes_to_h8(rk[i].x, rk[i].y);
+        *reinterpret_cast<f16x8_t*>(b + (k_put[i] ^ 16)) = codes_to_h8(rk[i].z, rk[i].w);
+      }
+      if (has_v) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = rv[j] ^ 0x80808080u;
+        char* v = b + v_put[0];
+        char* v2 = b + v_put[1];
+        *reinterpret_cast<uint4*>(v) = make_uint4(codes_pair<0>(w[0], w[1]), codes_pair<0>(w[2], w[3]), codes_pair<0>(w[4], w[5]), codes_pair<0>(w[6], w[7]));
+        *reinterpret_cast<uint4*>(v + 128) = make_uint4(codes_pair<1>(w[0], w[1]), codes_pair<1>(w[2], w[3]), codes_pair<1>(w[4], w[5]), codes_pair<1>(w[6], w[7]));
+        *reinterpret_cast<uint4*>(v2 + 256) = make_uint4(codes_pair<2>(w[0], w[1]), codes_pair<2>(w[2], w[3]), codes_pair<2>(w[4], w[5]), codes_pair<2>(w[6], w[7]));
+        *reinterpret_cast<uint4*>(v2 + 384) = make_uint4(codes_pair<3>(w[0], w[1]), codes_pair<3>(w[2], w[3]), codes_pair<3>(w[4], w[5]), codes_pair<3>(w[6], w[7]));
+      }
+      float* sc = reinterpret_cast<float*>(b + KB + VB);
+      if (tid < 128) sc[tid] = __uint_as_float(rs);
+      if (tid >= 64 && tid < 128) sc[64 + tid] = scale_exponent(__uint_as_float(rs));
+    };
+
+    if (kend > 0) fetch(0);                // in flight while the queries are read
     f16x8_t qf[2][NP][KS];
     float unit[2], M[2], l[2];
     int limit[2];
@@ -444,71 +526,44 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int r = wfirst + t * 16 + li;
-      unit[t] = load_query<T, HD, NP>(a, s, kvh, r, rows, lg, qf[t]);
+      unit[t] = load_query<T, HD, NP, true>(a, s, kvh, r, rows, lg, qf[t]);
       limit[t] = r <= last ? row_limit(a, s, r) : kend;
       M[t] = -INFINITY; l[t] = 0.f;
 #pragma unroll
       for (int e = 0; e < NE; ++e) o[t][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // this thread's share of 64 positions: KL pieces of K; 8 positions x 4 dimensions of V (HD = 64: half of the threads); one scale
-    uint4 rk[KL];
-    uint32_t rv[8];
-    float rs = 0.f;
-    const int vd = tid % (HD / 4), vg = tid / (HD / 4);                            // V: dimensions 4 vd .., positions 8 vg ..
-    auto fetch = [&](int kt) __attribute__((always_inline)) {
+    // this lane's place in the buffers.  Pieces are swapped within their rows (K: 16 pieces of a 256-byte row or 8 of a 128-byte one; V: 8)
+    // so that the 16 lanes that LDS serves together (0-3, 12-15, 20-27 and so on) reach different banks
+    int k_at[KS], v_at[2];
 #pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const int u = i * 256 + tid, key = min(kt + u / (HD / 16), kend - 1);
-        rk[i] = *reinterpret_cast<const uint4*>(kp + (int64_t)key * HD + (u % (HD / 16)) * 16);
-      }
-      if (HD == 128 || vg < 8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) rv[j] = *reinterpret_cast<const uint32_t*>(vp + (int64_t)min(kt + vg * 8 + j, kend - 1) * HD + vd * 4);
-      }
-      if (tid < 128) rs = (tid < 64 ? ksp : vsp)[min(kt + (tid & 63), kend - 1)];
-    };
-    auto put = [&](int buf) __attribute__((always_inline)) {
-      char* b = lds_t + buf * BUF;
-#pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const int u = i * 256 + tid, key = u / (HD / 16), c = (u % (HD / 16)) * 2;
-        // the row this position has in the first product's operand
-        const int row = (key >> 5) * 32 + ((key >> 2) & 1) * 16 + ((key >> 3) & 3) * 4 + (key & 3);
-        const int x = row & (HD / 8 - 1);
-        *reinterpret_cast<f16x8_t*>(b + row * (HD * 2) + ((c ^ x) << 4)) = codes_to_h8(rk[i].x, rk[i].y);
-        *reinterpret_cast<f16x8_t*>(b + row * (HD * 2) + (((c + 1) ^ x) << 4)) = codes_to_h8(rk[i].z, rk[i].w);
-      }
-      if (HD == 128 || vg < 8) {
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = rv[j] ^ 0x80808080u;
-        char* v = b + KB + vd * 4 * 128 + ((vg ^ (vd & 7)) << 4);
-        *reinterpret_cast<uint4*>(v) = make_uint4(codes_pair<0>(w[0], w[1]), codes_pair<0>(w[2], w[3]), codes_pair<0>(w[4], w[5]), codes_pair<0>(w[6], w[7]));
-        *reinterpret_cast<uint4*>(v + 128) = make_uint4(codes_pair<1>(w[0], w[1]), codes_pair<1>(w[2], w[3]), codes_pair<1>(w[4], w[5]), codes_pair<1>(w[6], w[7]));
-        *reinterpret_cast<uint4*>(v + 256) = make_uint4(codes_pair<2>(w[0], w[1]), codes_pair<2>(w[2], w[3]), codes_pair<2>(w[4], w[5]), codes_pair<2>(w[6], w[7]));
-        *reinterpret_cast<uint4*>(v + 384) = make_uint4(codes_pair<3>(w[0], w[1]), codes_pair<3>(w[2], w[3]), codes_pair<3>(w[4], w[5]), codes_pair<3>(w[6], w[7]));
-      }
-      float* sc = reinterpret_cast<float*>(b + KB + VB);
-      if (tid < 128) sc[tid] = rs;
-      if (tid >= 64 && tid < 128) sc[64 + tid] = scale_exponent(rs);
-    };
-
-    // 32 positions: half h of the buffer's 64
-    auto tile = [&](const int kt, const int buf, const int h, auto masked_tag) __attribute__((always_inline)) {
+    for (int c = 0; c < KS; ++c) k_at[c] = li * (HD * 2) + (((c * 4 + lg) ^ (li & (HD / 8 - 1))) << 4);
+    v_at[0] = KB + li * 128 + ((lg ^ (li >> 1)) << 4);
+    v_at[1] = v_at[0] ^ 64;
+    // 32 positions: half H of the buffer's 64
+    auto tile = [&](const int kt, const int buf, auto half_tag, auto masked_tag) __attribute__((always_inline)) {
+      constexpr int H = decltype(half_tag)::value;
       constexpr bool MASKED = decltype(masked_tag)::value;
       const char* b = lds_t + buf * BUF;
-      const float* sc = reinterpret_cast<const float*>(b + KB + VB) + h * 32 + lg * 8;
-      const int key0 = kt + h * 32 + lg * 8;
+      float ks[8], vs[8], ex[8];
+      {
+        const float* sc = reinterpret_cast<const float*>(b + KB + VB) + H * 32 + lg * 8;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          *reinterpret_cast<float4*>(ks + j) = *reinterpret_cast<const float4*>(sc + j);
+          *reinterpret_cast<float4*>(vs + j) = *reinterpret_cast<const float4*>(sc + 64 + j);
+          *reinterpret_cast<float4*>(ex + j) = *reinterpret_cast<const float4*>(sc + 128 + j);
+        }
+      }
+      const int key0 = kt + H * 32 + lg * 8;
       f32x4_t st[2][2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         st[0][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         st[1][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        const int row = h * 32 + kb * 16 + li;
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
-          const f16x8_t kf = *reinterpret_cast<const f16x8_t*>(b + row * (HD * 2) + (((lg * KS + c) ^ (li & (HD / 8 - 1))) << 4));
+          const f16x8_t kf = *reinterpret_cast<const f16x8_t*>(b + k_at[c] + (H * 32 + kb * 16) * (HD * 2));
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -521,9 +576,9 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
         float x[8], top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          x[j] = st[t][j >> 2][j & 3] * sc[j] * unit[t];
+          x[j] = st[t][j >> 2][j & 3] * ks[j];
           const bool in = !MASKED || key0 + j < limit[t];
-          top = fmaxf(top, in ? x[j] + sc[128 + j] : -INFINITY);
+          top = fmaxf(top, in ? fmaf(x[j], unit[t], ex[j]) : -INFINITY);
         }
         top = quad_max(top);
         if (top > M[t] + kSlack) {
@@ -539,9 +594,9 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool in = !MASKED || key0 + j < limit[t];
-          const float p = in ? __builtin_amdgcn_exp2f(x[j] - m) : 0.f;
+          const float p = in ? __builtin_amdgcn_exp2f(fmaf(x[j], unit[t], -m)) : 0.f;
           l[t] += p;
-          const float w = in ? p * sc[64 + j] : 0.f;
+          const float w = in ? p * vs[j] : 0.f;
           const f16_t hi = f2h(w);
           pf[t][0][j] = hi;
           if constexpr (NW == 2) pf[t][1][j] = f2h(w - h2f(hi));
@@ -549,8 +604,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
       }
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
-        const int d = e * 16 + li;
-        const f16x8_t vf = *reinterpret_cast<const f16x8_t*>(b + KB + d * 128 + (((h * 4 + lg) ^ ((d >> 2) & 7)) << 4));
+        const f16x8_t vf = *reinterpret_cast<const f16x8_t*>(b + v_at[H] + e * 2048);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -559,17 +613,16 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
     };
 
     __syncthreads();                       // the block before has read its last buffer
-    if (kend > 0) { fetch(0); put(0); }
+    if (kend > 0) put(0);
     __syncthreads();
     int buf = 0;
     for (int kt = 0; kt < kend; kt += 64, buf ^= 1) {
       const bool more = kt + 64 < kend;
       if (more) fetch(kt + 64);
-#pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        if (kt + h * 32 + 32 <= every) tile(kt, buf, h, std::false_type{});
-        else if (kt + h * 32 < wend) tile(kt, buf, h, std::true_type{});
-      }
+      if (kt + 32 <= every) tile(kt, buf, std::integral_constant<int, 0>{}, std::false_type{});
+      else if (kt < wend) tile(kt, buf, std::integral_constant<int, 0>{}, std::true_type{});
+      if (kt + 64 <= every) tile(kt, buf, std::integral_constant<int, 1>{}, std::false_type{});
+      else if (kt + 32 < wend) tile(kt, buf, std::integral_constant<int, 1>{}, std::true_type{});
       if (more) put(buf ^ 1);
       __syncthreads();
     }
@@ -578,13 +631,14 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
       const float sum = quad_sum(l[t]);
       const int r = wfirst + t * 16 + li;
       if (r > last) continue;
-      const float inv = limit[t] > 0 ? 1.f / sum : 0.f;
-      T* out = reinterpret_cast<T*>(a.out) + (int64_t)(s.first + r / a.per) * a.ldo + (kvh * a.per + r % a.per) * HD + lg * 4;
+      const float inv = limit[t] > 0 ? 1.f / sum : 0.f;      // a row that sees nothing has added nothing: zeros
+      const int t1 = over_per(a, r);
+      T* out = reinterpret_cast<T*>(a.out) + (int64_t)(s.first + t1) * a.ldo + (kvh * a.per + r - t1 * a.per) * HD + lg * 4;
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = limit[t] > 0 ? o[t][e][i] * inv : 0.f;
+        for (int i = 0; i < 4; ++i) v[i] = o[t][e][i] * inv;
         st_out<T, 4>(out + e * 16, v);
       }
     }
@@ -665,12 +719,12 @@ int launch_read(const wj_kv8* c, const wj_kv8_batch* b, int dtype, void* k, int6
 }
 
 // Rows per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).
-struct AttnPlan { int rt, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel
+struct AttnPlan { int rt, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel (16-bit types; float32 rows take two blocks)
 AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
   const int per = n_heads / c.heads;
   const int64_t rows = (int64_t)(b.max_new > 0 ? b.max_new : 1) * per;
   AttnPlan p;
-  if (rows > 64 && (int64_t)b.seqs * c.heads * ((rows + 127) / 128) >= 128) return {0, 1, 0};
+  if (rows > 64 && (int64_t)c.ctx * c.dim < 0x7fff0000 && (int64_t)b.seqs * c.heads * ((rows + 127) / 128) >= 128) return {0, 1, 0x40000000};
   p.rt = rows <= 16 ? 1 : 2;
   const int64_t groups = (int64_t)b.seqs * c.heads * ((rows + 16 * p.rt - 1) / (16 * p.rt));
   const int len = b.max_len < c.ctx ? (b.max_len > 0 ? b.max_len : 1) : c.ctx;
@@ -710,7 +764,9 @@ int start_tile(const AttnArgs& a, hipStream_t s) {
 }
 template <int HD, typename T>
 int pick_rows(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-  if (p.rt == 0) return start_tile<T, HD>(a, s);
+  if (p.rt == 0) {
+    if constexpr (sizeof(T) == 2) return start_tile<T, HD>(a, s);
+  }
   return p.rt == 1 ? start_attention<T, HD, 1>(a, s) : start_attention<T, HD, 2>(a, s);
 }
 template <int HD>
@@ -764,7 +820,7 @@ int wj_kv8_attention(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch
   if (batch->seqs == 0 || batch->rows == 0) return WJ_OK;
   WJ_REQUIRE((int64_t)cache->slots * cache->ctx > 0, "wj_kv8_attention: an empty cache");
   WJ_REQUIRE(q_dev && out_dev, "wj_kv8_attention: NULL argument");
-  WJ_REQUIRE((int64_t)batch->rows * n_heads < ((int64_t)1 << 31) - 4096, "wj_kv8_attention: %d rows of %d heads", batch->rows, n_heads);
+  WJ_REQUIRE((int64_t)batch->rows * n_heads < (int64_t)1 << 28, "wj_kv8_attention: %d rows of %d heads (below 2^28 in all)", batch->rows, n_heads);
   WJ_REQUIRE(ldq >= 0 && (batch->rows == 1 || ldo >= (int64_t)n_heads * cache->dim), "wj_kv8_attention: output rows overlap");
   const int64_t need = wj_kv8_attention_workspace(ctx, cache, batch, n_heads);
   WJ_REQUIRE(workspace_bytes >= need && (workspace_dev || need == 0), "wj_kv8_attention: %lld bytes of workspace, %lld needed", (long long)workspace_bytes, (long long)need);
@@ -772,8 +828,9 @@ int wj_kv8_attention(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch
   DeviceScope dev;
   WJ_HIP(dev.enter(ctx->device));
   const AttnPlan p = plan_attention(*cache, *batch, n_heads);
-  AttnArgs a{Kv8Args{*cache, *batch}, q_dev, ldq, out_dev, ldo, n_heads, n_heads / cache->heads, causal, fabsf(scale) * 1.44269504088896340736f,
-             scale < 0.f ? -1.f : 1.f, p.chunk, p.nsplit, reinterpret_cast<float*>(workspace_dev), nullptr};
+  AttnArgs a{Kv8Args{*cache, *batch}, q_dev, ldq, out_dev, ldo, n_heads, n_heads / cache->heads, causal, 0, scale * 1.44269504088896340736f,
+             p.chunk, p.nsplit, reinterpret_cast<float*>(workspace_dev), nullptr};
+  if (a.per > 1) a.per_inv = (uint32_t)((((uint64_t)1 << 32) + a.per - 1) / a.per);
   a.ml = reinterpret_cast<float2*>(a.part + (int64_t)batch->rows * n_heads * p.nsplit * cache->dim);
   hipStream_t s = ctx->pick(stream);
   if (cache->dim == 128) return pick_type<128>(a, p, dtype, s);
