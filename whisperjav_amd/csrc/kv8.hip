@@ -453,16 +453,20 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
   constexpr int KL = HD / 64;                                                      // 16-byte pieces of K per thread
   extern __shared__ __attribute__((aligned(16))) char lds_t[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
-  // workgroups go to the 8 XCDs in turn: all row blocks of one (sequence, head) on one XCD, the longest first
-  const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3, group = idx / blocks * 8 + xcd;
-  if (group >= a.s.b.seqs * a.s.c.heads) return;
+  // Workgroups go to the 8 XCDs in turn: all row blocks of one (sequence, head) on one XCD.  Under a causal mask later blocks see more: the
+  // last blocks of every (sequence, head) come first, so that short ones fill the end.
+  const int groups = a.s.b.seqs * a.s.c.heads, per_xcd = (groups + 7) >> 3;
+  const int xcd = blockIdx.x & 7, idx = blockIdx.x >> 3, rank = idx / per_xcd, group = (idx - rank * per_xcd) * 8 + xcd;
+  if (group >= groups) return;
   const int seq = group / a.s.c.heads, kvh = group - seq * a.s.c.heads;
   const Span s = span_of(a.s, seq);
   const int rows = s.n * a.per, n_blocks = (rows + 127) >> 7;
   const int64_t row0 = ((int64_t)max(s.slot, 0) * a.s.c.heads + kvh) * a.s.c.ctx;
   const auto k_buf = buffer_of(a.s.c.k_dev + row0 * HD, a.s.c.ctx * HD), v_buf = buffer_of(a.s.c.v_dev + row0 * HD, a.s.c.ctx * HD);
   const auto ks_buf = buffer_of(a.s.c.k_scale_dev + row0, a.s.c.ctx * 4), vs_buf = buffer_of(a.s.c.v_scale_dev + row0, a.s.c.ctx * 4);
-  for (int block = n_blocks - 1 - idx % blocks; block >= 0; block -= blocks) {
+  // (a sequence of fewer blocks sits out the first ranks; one of more than `blocks` takes several)
+  for (int block = n_blocks > blocks ? n_blocks - 1 - rank : blocks - 1 - rank; block >= 0; block -= blocks) {
+    if (block >= n_blocks) break;
     const int first = block * 128, last = min(rows, first + 128) - 1;
     const int wfirst = first + wave * 32, wlast = min(last, wfirst + 31);
     const int kend = row_limit(a, s, last);                                        // positions the workgroup walks
