@@ -161,6 +161,21 @@ def test_gemm_layers(q8, m, n, k, dtype, bias):
     check_gemm(q8, rng(m + n + k), m, n, k, dtype, bias, ((-k % 16, 0),))
 
 
+@pytest.mark.parametrize("dtype,m,n", [(torch.float32, 8200, 8301), (torch.bfloat16, 16397, 8301)])
+def test_gemm_output_beyond_the_caches(q8, dtype, m, n):
+    """an output of more than 256 MiB takes other stores: the same bits as its parts computed alone, and the formula's values"""
+    k, g = 130, rng(m)
+    a, w = strided(int8(g, m, k), 14), strided(int8(g, n, k), 14)
+    sa, sw = torch.rand(m, generator=g) * 0.02, torch.rand(n, generator=g) * 0.02
+    got = q8.gemm(a, sa.cuda(), w, sw.cuda(), dtype=dtype)
+    for lo in range(0, m, 2050):
+        part = slice(lo, min(m, lo + 2050))
+        assert torch.equal(got[part], q8.gemm(a[part], sa[part].cuda(), w, sw.cuda(), dtype=dtype)), lo
+    rows = torch.tensor([0, 1, 255, 256, m // 2, m - 2, m - 1])
+    want = ref.gemm(a[rows.cuda()].cpu(), sa[rows], w.cpu(), sw)
+    assert bool(((got[rows.cuda()].cpu().double() - want).abs() <= 4 * E * want.abs() + (U[dtype] + E) * want.abs() + TINY[dtype]).all())
+
+
 def test_gemm_largest_sum_is_exact(q8):
     k = 131071
     a = torch.full((3, k), -128, dtype=torch.int8)

@@ -206,6 +206,7 @@ __global__ __launch_bounds__(256) void q8_dequantize_kernel(const int8_t* __rest
 // side, which is enough.  int32 sums are exact, so the kernels agree bit for bit whatever their order.
 // --------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 
 struct GemmQ8Args {
   const int8_t* a; int64_t lda; const float* sa;
@@ -254,9 +255,16 @@ template <typename T> __device__ __forceinline__ uint32_t pack_any(float lo, flo
   return (uint32_t)__builtin_bit_cast(uint16_t, to_T<T>(lo)) | ((uint32_t)__builtin_bit_cast(uint16_t, to_T<T>(hi)) << 16);
 }
 
+// 16 bytes of output, at any element alignment; PAST: past the caches
+template <bool PAST> __device__ __forceinline__ void st16(void* p, u32x4_t w) {
+  typedef uint32_t at2_t __attribute__((ext_vector_type(4), aligned(2)));
+  if constexpr (PAST) __builtin_nontemporal_store((at2_t)w, reinterpret_cast<at2_t*>(p));
+  else *reinterpret_cast<at2_t*>(p) = w;
+}
+
 // out = acc * (sa * sw) + bias of RI x 4 fragments of 16 x 16, wave origin (mw, nw).  16-bit types: lanes 16 apart trade halves of
 // neighbouring fragments (v_permlane16_swap), so that a lane stores 8 consecutive columns at once.
-template <typename T, int RI>
+template <typename T, bool PAST, int RI>
 __device__ __forceinline__ void q8_epilogue(const GemmQ8Args& g, int64_t mw, int nw, int lane, i32x4_t (&acc)[RI][4]) {
   const int li = lane & 15, q = lane >> 4;
   float sw[4][4], bias[4][4];
@@ -284,7 +292,7 @@ __device__ __forceinline__ void q8_epilogue(const GemmQ8Args& g, int64_t mw, int
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * (sa[i] * sw[j][e]) + bias[j][e];
         if (m < g.m) {
-          if (n + 4 <= g.n) __builtin_memcpy(row + n, v, 16);
+          if (n + 4 <= g.n) st16<PAST>(row + n, u32x4_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
           else
 #pragma unroll
             for (int e = 0; e < 3; ++e)
@@ -304,10 +312,10 @@ __device__ __forceinline__ void q8_epilogue(const GemmQ8Args& g, int64_t mw, int
         const uint32_t b0 = pack_any<T>(vb[0], vb[1]), b1 = pack_any<T>(vb[2], vb[3]);
         const auto s0 = __builtin_amdgcn_permlane16_swap(a0, b0, false, false);
         const auto s1 = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
-        const uint32_t w[4] = {(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
+        const u32x4_t w = {(uint32_t)s0[0], (uint32_t)s1[0], (uint32_t)s0[1], (uint32_t)s1[1]};
         const int n8 = nw + (jp + (q & 1)) * 16 + (q >> 1) * 8;
         if (m < g.m) {
-          if (n8 + 8 <= g.n) __builtin_memcpy(row + n8, w, 16);
+          if (n8 + 8 <= g.n) st16<PAST>(row + n8, w);
           else
 #pragma unroll
             for (int e = 0; e < 7; ++e)
@@ -336,7 +344,7 @@ __device__ __forceinline__ void tile_of(int lin, int nx, int ny, int* tx, int* t
 // WAR: the other buffer held pair p - 1, read last in group 1's MEM(2p - 1), retired before B(4p - 1); MEM(2p) starts after it.
 // RAW: both groups have waited for pair p + 1 by B(4p + 3); it is first read after that.
 // 128-byte LDS rows, 16-byte piece c of row r in place c ^ (r & 7).
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, int nx, int ny) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [buffer][A | W][256][128]
   constexpr int STAGE = 2 * 256 * 128;
@@ -419,41 +427,44 @@ __global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, in
 #undef WJ_Q8_READ
 #undef WJ_Q8_CLEAR
 #undef WJ_Q8_MFMA
-  q8_epilogue<T, 8>(g, m0 + wm * 128, n0 + wn * 64, lane, acc);
+  q8_epilogue<T, PAST, 8>(g, m0 + wm * 128, n0 + wn * 64, lane, acc);
 }
 
-// 64 x 128 tile, k steps of 128 codes, a ring of 3 buffers with 2 steps requested ahead, two workgroups per CU.  Eight waves: (2 x 2, 32 x 64 each) twice,
+// BM x 128 tile, k steps of 128 codes, a ring of 3 buffers with 2 steps requested ahead (BM = 64: two workgroups per CU).  Eight waves: (2 x 2, BM / 2 x 64 each) twice,
 // each four taking one half of every step's codes, so that the two waves of a SIMD overlap one's LDS reads with the other's products; the
-// two halves' sums meet in LDS at the end, each four finishing 16 of every 32 rows.  For calls with too few 256-tiles to fill the chip;
+// two halves' sums meet in LDS at the end, each four finishing half of the rows.  For calls with too few 256-tiles to fill the chip;
 // ksplit > 1: slices of k on the grid's second axis write raw sums, joined by q8_gemm_join_kernel.
-template <typename T>
+template <typename T, int BM>
 __global__ __launch_bounds__(512) void q8_gemm_tile_kernel(const GemmQ8Args g, int nx, int ny) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [stage][A: 64 | W: 128][128]
-  constexpr int NS = 3, STAGE = (64 + 128) * 128;
+  constexpr int NS = 3, STAGE = (BM + 128) * 128, RI = BM / 32, QA = BM / 64;      // 16-row blocks and requests of a wave
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
   int tx, ty;
   tile_of(blockIdx.x, nx, ny, &tx, &ty);
-  const int64_t m0 = (int64_t)ty * 64;
+  const int64_t m0 = (int64_t)ty * BM;
   const int n0 = tx * 128;
   const int steps = (g.k + 127) / 128;
   const int s_begin = (int)((int64_t)steps * blockIdx.y / g.ksplit), s_end = (int)((int64_t)steps * (blockIdx.y + 1) / g.ksplit);
   const int nk = s_end - s_begin;
   const int c = (lane & 7) ^ ((lane >> 3) & 7);
-  const int8_t* ga = g.a + min(m0 + wave * 8 + (lane >> 3), g.m - 1) * g.lda + c * 16 + (int64_t)s_begin * 128;
+  const int8_t* ga[QA];
+#pragma unroll
+  for (int q = 0; q < QA; ++q) ga[q] = g.a + min(m0 + (wave * QA + q) * 8 + (lane >> 3), g.m - 1) * g.lda + c * 16 + (int64_t)s_begin * 128;
   const int8_t* gw0 = g.w + (int64_t)min(n0 + wave * 16 + (lane >> 3), g.n - 1) * g.ldw + c * 16 + (int64_t)s_begin * 128;
   const int8_t* gw1 = g.w + (int64_t)min(n0 + wave * 16 + 8 + (lane >> 3), g.n - 1) * g.ldw + c * 16 + (int64_t)s_begin * 128;
   auto issue = [&](int s, int buf) __attribute__((always_inline)) {
     const int back = s == steps - 1 && s * 128 + c * 16 >= g.k ? s * 128 + c * 16 : 0;
-    dma16(ga - back, &lds[buf * STAGE + wave * 1024]);
-    dma16(gw0 - back, &lds[buf * STAGE + 64 * 128 + wave * 2048]);
-    dma16(gw1 - back, &lds[buf * STAGE + 64 * 128 + wave * 2048 + 1024]);
-    ga += 128; gw0 += 128; gw1 += 128;
-  };
-  i32x4_t acc[2][4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int q = 0; q < QA; ++q) { dma16(ga[q] - back, &lds[buf * STAGE + (wave * QA + q) * 1024]); ga[q] += 128; }
+    dma16(gw0 - back, &lds[buf * STAGE + BM * 128 + wave * 2048]);
+    dma16(gw1 - back, &lds[buf * STAGE + BM * 128 + wave * 2048 + 1024]);
+    gw0 += 128; gw1 += 128;
+  };
+  i32x4_t acc[RI][4];
+#pragma unroll
+  for (int i = 0; i < RI; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
 #pragma unroll
@@ -462,57 +473,64 @@ __global__ __launch_bounds__(512) void q8_gemm_tile_kernel(const GemmQ8Args g, i
   const int off = (lane & 15) * 128 + (((half * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
   int buf = 0;
   for (int kt = 0; kt < nk; ++kt) {
-    const int younger = min(NS - 2, nk - 1 - kt);      // steps requested after kt (3 requests each) that may stay in flight
-    if (younger >= 1) asm volatile("s_waitcnt vmcnt(3)" ::: "memory");
+    // the step after kt may stay in flight
+    if (kt + 1 < nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(QA + 2) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // step kt is visible to all; the buffer of step kt - 1 is free (its reads were retired before this barrier)
     q8_barrier();
     if (kt + NS - 1 < nk) issue(s_begin + kt + NS - 1, buf == 0 ? NS - 1 : buf - 1);
-    const int8_t* la = &lds[buf * STAGE + wm * 32 * 128 + off];
-    const int8_t* lw = &lds[buf * STAGE + 64 * 128 + wn * 64 * 128 + off];
-    i32x4_t af[2], wf[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) af[i] = *reinterpret_cast<const i32x4_t*>(la + i * 2048);
+    const int8_t* la = &lds[buf * STAGE + wm * (BM / 2) * 128 + off];
+    const int8_t* lw = &lds[buf * STAGE + BM * 128 + wn * 64 * 128 + off];
+    i32x4_t af[RI], wf[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) wf[j] = *reinterpret_cast<const i32x4_t*>(lw + j * 2048);
+#pragma unroll
+    for (int i = 0; i < RI; ++i) af[i] = *reinterpret_cast<const i32x4_t*>(la + i * 2048);
     if (s_begin + kt == steps - 1 && (g.k & 127)) {
       const i32x4_t mask = piece_mask(g.k - ((s_begin + kt) * 128 + half * 64 + (lane >> 4) * 16));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) af[i] &= mask;
+      for (int i = 0; i < RI; ++i) af[i] &= mask;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < RI; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(wf[j], af[i], acc[i][j]);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     buf = buf == NS - 1 ? 0 : buf + 1;
   }
-  // this half finishes rows 16 half .. of the wave's 32 and hands the others over
+  // this half finishes one half of the wave's rows and hands the others over
   __syncthreads();
   i32x4_t* swap = reinterpret_cast<i32x4_t*>(lds);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) swap[(wave * 4 + j) * 64 + lane] = half ? acc[0][j] : acc[1][j];
-  __syncthreads();
-  i32x4_t sum[1][4];
+  for (int i = 0; i < RI / 2; ++i)
 #pragma unroll
-  for (int j = 0; j < 4; ++j) sum[0][j] = (half ? acc[1][j] : acc[0][j]) + swap[((wave ^ 4) * 4 + j) * 64 + lane];
-  const int64_t mw = m0 + wm * 32 + half * 16;
+    for (int j = 0; j < 4; ++j) swap[((wave * (RI / 2) + i) * 4 + j) * 64 + lane] = half ? acc[i][j] : acc[RI / 2 + i][j];
+  __syncthreads();
+  i32x4_t sum[RI / 2][4];
+#pragma unroll
+  for (int i = 0; i < RI / 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[i][j] = (half ? acc[RI / 2 + i][j] : acc[i][j]) + swap[(((wave ^ 4) * (RI / 2) + i) * 4 + j) * 64 + lane];
+  const int64_t mw = m0 + wm * (BM / 2) + half * (BM / 4);
   const int nw = n0 + wn * 64;
   if (g.ksplit == 1) {
-    q8_epilogue<T, 1>(g, mw, nw, lane, sum);
+    q8_epilogue<T, false, RI / 2>(g, mw, nw, lane, sum);
     return;
   }
-  const int64_t m = mw + (lane & 15);
-  if (m >= g.m) return;
-  int32_t* row = g.slab + ((int64_t)blockIdx.y * g.m + m) * g.n;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int n = nw + j * 16 + (lane >> 4) * 4;
-    if (n + 4 <= g.n) __builtin_memcpy(row + n, &sum[0][j], 16);
-    else
+  for (int i = 0; i < RI / 2; ++i) {
+    const int64_t m = mw + i * 16 + (lane & 15);
+    if (m >= g.m) continue;
+    int32_t* row = g.slab + ((int64_t)blockIdx.y * g.m + m) * g.n;
 #pragma unroll
-      for (int e = 0; e < 3; ++e)
-        if (n + e < g.n) row[n + e] = sum[0][j][e];
+    for (int j = 0; j < 4; ++j) {
+      const int n = nw + j * 16 + (lane >> 4) * 4;
+      if (n + 4 <= g.n) __builtin_memcpy(row + n, &sum[i][j], 16);
+      else
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (n + e < g.n) row[n + e] = sum[i][j][e];
+    }
   }
 }
 
@@ -693,14 +711,19 @@ int launch_rows(wj_ctx* ctx, int dtype, int delta_dtype, const RowArgs& a, void*
 //     that is at most 36 MiB;
 //   tile / big: 2048 x 4096 x 2048 27.6 / 29.6, 3000 x 2048 x 6144 53 / 67, 512 x 12288 x 2048 22 / 30, 1024 x 12288 x 2048 40 / 32,
 //     3000 x 4096 x 2048 39 / 31, 1500 x 12288 x 2048 58 / 58: a round of 256 big tiles, filled or not, takes as long as 1000 small ones;
+//   tile of 64 / 128 rows: 512 x 5176 x 5824 39 / 31, 3000 x 1190 x 3808 31 / 25, 240 x 12288 x 2048 15.6 / 15.2, 384 x 5176 x 5824 24 / 31, 512 x
+//     12288 x 2048 22.6 / 26.9: the larger pays where small ones would share CUs unevenly and large ones have a CU each;
+//   big, stores past the caches: 16384 x 12288 x 2048 (402 MB out) 440 -> 398, 8192 x 12288 x 2048 (201 MB) 188 -> 208: for outputs beyond the
+//     256 MiB of the memory-side cache;
 //   tile, slices 1 / 2 / 4: 100 x 4096 x 2048 10.0 / 11.1 / 11.6, 100 x 2048 x 6144 23 / 15 / 12.5, 512 x 2048 x 6144 22.5 / 19.1 / 19.8: a
 //     slice saves its share of the 0.4 us that a step takes and the join costs 3 us, so it pays from 16 steps a slice while CUs are idle.
-enum GemmKind { GEMM_ROWS, GEMM_BIG, GEMM_TILE };
+enum GemmKind { GEMM_ROWS, GEMM_BIG, GEMM_TILE, GEMM_TILE128 };
 struct GemmPlan { GemmKind kind; int ksplit; };
 GemmPlan plan_gemm(int64_t m, int n, int k) {
   if (m <= 16 || (m <= 64 && m * k * ((n + 15) / 16) <= (int64_t)36 << 20)) return {GEMM_ROWS, 1};
   const int64_t t256 = ((m + 255) / 256) * ((n + 255) / 256), t64 = ((m + 63) / 64) * ((n + 127) / 128);
   if (t64 > 1000 * ((t256 + 255) / 256)) return {GEMM_BIG, 1};
+  if (t64 > 256 && ((m + 127) / 128) * ((n + 127) / 128) <= 256) return {GEMM_TILE128, 1};
   const int steps = (k + 127) / 128;
   int ks = 1;
   while (ks < 8 && t64 * ks * 2 <= 256 && steps > 16 * ks) ks *= 2;
@@ -716,18 +739,29 @@ int allow_lds(K kernel, AttrOnce& once, int bytes) {
   return WJ_OK;
 }
 
-template <typename T>
+template <typename T, int BM>
 int start_tile(const GemmQ8Args& g, hipStream_t s) {
   static AttrOnce once;
-  constexpr int lds = 3 * (64 + 128) * 128;
-  if (int rc = allow_lds(q8_gemm_tile_kernel<T>, once, lds)) return rc;
-  const int nx = (g.n + 127) / 128, ny = (int)((g.m + 63) / 64);
-  hipLaunchKernelGGL((q8_gemm_tile_kernel<T>), dim3((unsigned)nx * ny, g.ksplit), dim3(512), lds, s, g, nx, ny);
+  constexpr int lds = 3 * (BM + 128) * 128;
+  if (int rc = allow_lds(q8_gemm_tile_kernel<T, BM>, once, lds)) return rc;
+  const int nx = (g.n + 127) / 128, ny = (int)((g.m + BM - 1) / BM);
+  hipLaunchKernelGGL((q8_gemm_tile_kernel<T, BM>), dim3((unsigned)nx * ny, g.ksplit), dim3(512), lds, s, g, nx, ny);
   WJ_LAUNCH_CHECK();
   if (g.ksplit > 1) {
     hipLaunchKernelGGL(q8_gemm_join_kernel<T>, dim3((unsigned)((g.n + 1023) / 1024), (unsigned)g.m), dim3(256), 0, s, g);
     WJ_LAUNCH_CHECK();
   }
+  return WJ_OK;
+}
+
+template <typename T, bool PAST>
+int start_big(const GemmQ8Args& g, hipStream_t s) {
+  static AttrOnce once;
+  constexpr int lds = 2 * 2 * 256 * 128;
+  if (int rc = allow_lds(q8_gemm_big_kernel<T, PAST>, once, lds)) return rc;
+  const int nx = (g.n + 255) / 256, ny = (int)((g.m + 255) / 256);
+  hipLaunchKernelGGL((q8_gemm_big_kernel<T, PAST>), dim3((unsigned)nx * ny), dim3(512), lds, s, g, nx, ny);
+  WJ_LAUNCH_CHECK();
   return WJ_OK;
 }
 
@@ -744,16 +778,9 @@ int launch_gemm_q8(GemmQ8Args g, hipStream_t s) {
       WJ_LAUNCH_CHECK();
       return WJ_OK;
     }
-    case GEMM_BIG: {
-      static AttrOnce once;
-      constexpr int lds = 2 * 2 * 256 * 128;
-      if (int rc = allow_lds(q8_gemm_big_kernel<T>, once, lds)) return rc;
-      const int nx = (g.n + 255) / 256, ny = (int)((g.m + 255) / 256);
-      hipLaunchKernelGGL(q8_gemm_big_kernel<T>, dim3((unsigned)nx * ny), dim3(512), lds, s, g, nx, ny);
-      WJ_LAUNCH_CHECK();
-      return WJ_OK;
-    }
-    default: return start_tile<T>(g, s);
+    case GEMM_BIG: return g.m * g.n * (int64_t)sizeof(T) > (int64_t)256 << 20 ? start_big<T, true>(g, s) : start_big<T, false>(g, s);
+    case GEMM_TILE128: return start_tile<T, 128>(g, s);
+    default: return start_tile<T, 64>(g, s);
   }
 }
 
