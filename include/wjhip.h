@@ -483,13 +483,15 @@ int wj_comm_destroy(wj_comm* comm);
  * The operators of a decoder layer whose products run on 8-bit integers and whose key / value cache holds 8-bit codes: the
  * precision CTranslate2 offers the reference as compute_type="int8" (whisperjav/modules/faster_whisper_pro_asr.py:247-253 passes
  * compute_type on; weights in int8, activations quantised per row as they are produced), plus the cache.
- * A ROW of values x is held as int8 codes in [-127, 127] and one float32 scale: scale = max |x| / 127, code = x * (127 / max |x|)
- * rounded to nearest, ties to even; x reads back as code * scale, off by at most scale / 2.  A row of zeros has scale 0.  A row that
- * holds a NaN or an infinity has scale NaN and codes 0, so that it reads back as NaN and stays a single row's matter.
+ * A ROW of values x is held as int8 codes in [-127, 127] and one float32 scale: scale = max |x| / 127, code = x / scale rounded to
+ * nearest, ties to even; x reads back as code * scale, off by at most scale / 2.  A row of zeros has scale 0.  A row that holds a NaN or
+ * an infinity has scale NaN and codes 0, so that it reads back as NaN and stays a single row's matter.
  * Every call is asynchronous on `stream` and may be captured into a graph (no allocation, no copy, no memset inside); `stream` =
  * WJ_STREAM_DEFAULT names the device's null stream (NULL is the context's own stream, as everywhere).  The caller's current device is
  * left as it was.  Strides (ld*) are in elements and count from row to row; elements of a row are contiguous.  Outputs must not overlap
- * inputs unless a parameter says so.  Calls with no rows do nothing.  wj_k_gemm_mx8 is the MX-fp8 relative. */
+ * inputs unless a parameter says so.  Calls with no rows do nothing.  No call keeps anything: two calls on two streams may run at once
+ * (each with its own workspace).  Their relatives among the kernel-level entry points below: wj_k_gemm, wj_k_gemm_mx8, wj_k_layernorm,
+ * wj_k_attention_dec.  whisperjav_amd/q8.py has them on torch tensors. */
 #define WJ_STREAM_DEFAULT ((void*)(intptr_t)-1)
 
 /* r = x + delta; y = r / sqrt(mean(r^2) + eps) * w; codes, scale = y quantised per row.  x, residual: `dtype`; delta (NULL: none):
@@ -545,7 +547,7 @@ int wj_kv8_write(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, in
 /* the same positions read back as values, [rows][heads][dim] in `dtype` */
 int wj_kv8_read(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int dtype, void* k_dev, int64_t ldk, void* v_dev, int64_t ldv,
                 void* stream);
-/* out[row][h] = softmax_j(scale * q[row][h] . k_j) v_j over the cached positions j of the row's sequence, j <= the row's own position
+/* out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j over the cached positions j of the row's sequence, j <= the row's own position
  * (causal != 0) or j < lens[b] (causal = 0: an encoder's states of another length, written once), the first ctx positions at most.
  * q, out [rows][n_heads][dim] in `dtype`; query head h reads key / value head h / (n_heads / heads), n_heads <= 16 heads.  A row that
  * sees no position (an empty cache, a causal row before position 0) is zeros.

@@ -312,6 +312,7 @@ LAYOUTS = {
     "one": ([1], [0, 1], [1]),
     "steps": ([3, 0, 1, 2], [0, 1, 2, 3, 4], [1, 64, 65, 200]),
     "ragged": ([2, 0, -1, 3, 1, 7], [0, 5, 5, 8, 24, 41, 42], [70, 3, 9, 16, 130, 4]),
+    "hundreds": ([4, 0], [0, 1, 4], [199, 180]),
     "short": ([0, 1, 2], [0, 4, 8, 20], [2, 0, 12]),                    # rows before position 0; an empty cache
     "past": ([0, 1], [0, 2, 5], [201, 260]),                             # lengths beyond the cache's 200 positions
     "prompt": ([1, 0, 3], [0, 150, 151, 351], [150, 1, 200]),
@@ -368,7 +369,7 @@ def test_attention_of_many_prompts(q8, dim, heads, per, dtype, causal):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("new,length", [(1, 5000), (3, 4099), (20, 3001), (70, 2500)])
+@pytest.mark.parametrize("new,length", [(1, 5000), (3, 4099), (20, 3001), (70, 2500), (1, 1000), (13, 777)])
 def test_attention_over_a_long_cache(q8, dtype, new, length):
     """few rows, many positions: the work is split over the positions and joined"""
     g = rng(length)
@@ -556,6 +557,11 @@ def test_refusals_on_the_device(q8):
         q8.quantize(x, swiglu_block=5)
     with pytest.raises(WjError):
         q8.rmsnorm(x, w, -1.0)
+    grad = torch.zeros(4, 64, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        q8.quantize(grad)
+    with torch.no_grad():
+        q8.quantize(grad)
     with pytest.raises(WjError):
         q8.quantize(torch.zeros(1, 32769).cuda())
     with pytest.raises(ValueError):

@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, T* __res
 // Attention over the cache.
 //
 // Per key / value head the rows of a sequence are its (new row, query head of the group) pairs, r = t * per + g; a workgroup takes
-// 16 RT of them and a range of positions, its four waves take 32 positions at a time in turn.  Codes go from memory straight into the
+// 16 RT of them and a range of positions, its waves (four, or eight) take 32 positions at a time in turn.  Codes go from memory straight into the
 // operands of the matrix cores: S^T = K Q^T per 16 positions, the positions of two such products permuted so that the weights leave the
 // first product in the order the second one, O^T += V^T P^T, wants them.  An int8 code is exact in float16 (byte | 0x6400 is 1024 + byte,
 // minus 1152), so the products lose nothing of the cache; the query is carried in units of a power of two that bounds its row, exact for
@@ -246,15 +246,15 @@ template <int N> struct Part {
   }
 };
 
-template <typename T, int HD, int RT>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv8_attn_rows_kernel(const AttnArgs a) {
+template <typename T, int HD, int RT, int NV>      // NV waves
+__global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv8_attn_rows_kernel(const AttnArgs a) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;                              // halves of a query
   constexpr int NW = std::is_same<T, bf16_t>::value ? 1 : 2;              // halves of a weight
   constexpr int NE = HD / 16;                  // 16-dim tiles of the output; a lane's output dims are NE consecutive ones, four times
   constexpr int KW = HD / 64;                  // 16-byte pieces of a key per lane
   constexpr int LDO = HD + 4;
-  __shared__ __attribute__((aligned(16))) float lo[4 * 16 * LDO];
-  __shared__ float2 lml[4 * 16];
+  __shared__ __attribute__((aligned(16))) float lo[NV * 16 * LDO];
+  __shared__ float2 lml[NV * 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
   const int kvh = blockIdx.y;
   const Span s = span_of(a.s, blockIdx.z);
@@ -395,12 +395,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv8_at
         value_tile(std::integral_constant<int, 6>{}); value_tile(std::integral_constant<int, 7>{});
       }
     };
-    for (int kt = kbeg + 32 * wave; kt < kend; kt += 128) {
+    for (int kt = kbeg + 32 * wave; kt < kend; kt += 32 * NV) {
       if (kt + 32 <= min(every, kend)) tile(kt, std::false_type{});
       else tile(kt, std::true_type{});
     }
 
-    // the four waves' parts meet in LDS, 16 rows at a time
+    // the waves' parts meet in LDS, 16 rows at a time
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       if (first + t * 16 > last) break;
@@ -415,12 +415,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv8_at
       }
       __syncthreads();
       const int row = tid >> 4, r = first + t * 16 + row, d0 = (tid & 15) * NE;
-      if (r <= last) {
+      if (tid < 256 && r <= last) {
         Part<NE> p;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) p.see(lml[w * 16 + row]);
+        for (int w = 0; w < NV; ++w) p.see(lml[w * 16 + row]);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) p.add(lml[w * 16 + row], &lo[(w * 16 + row) * LDO + d0]);
+        for (int w = 0; w < NV; ++w) p.add(lml[w * 16 + row], &lo[(w * 16 + row) * LDO + d0]);
         const int t1 = over_per(a, r);
         const int64_t at = s.first + t1, head = kvh * a.per + r - t1 * a.per;
         if (a.nsplit == 1) {
@@ -669,6 +669,9 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const AttnArgs a, in
   }
 }
 
+// the launch's sizes go by the hints as far as they can be true
+int most_new(const wj_kv8_batch& b) { return b.max_new < 1 ? 1 : b.max_new < b.rows ? b.max_new : b.rows; }
+
 int check_kv8(const char* who, wj_ctx* ctx, const wj_kv8* c, const wj_kv8_batch* b, int dtype) {
   WJ_REQUIRE(ctx && c && b, "%s: NULL argument", who);
   WJ_REQUIRE(known_dtype(dtype), "%s: unknown dtype %d", who, dtype);
@@ -722,32 +725,44 @@ int launch_read(const wj_kv8* c, const wj_kv8_batch* b, int dtype, void* k, int6
   return start_read<bf16_t, 64>(c, b, k, ldk, v, ldv, pairs, s);
 }
 
-// Rows per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).
-struct AttnPlan { int rt, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel (16-bit types; float32 rows take two blocks)
+// Rows and waves per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).
+struct AttnPlan { int rt, waves, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel (16-bit types; float32 rows take two blocks)
+constexpr int kWhole = 0x40000000;
 AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
   const int per = n_heads / c.heads;
-  const int64_t rows = (int64_t)(b.max_new > 0 ? b.max_new : 1) * per;
+  const int64_t rows = (int64_t)most_new(b) * per;
+  const int64_t tiles = (int64_t)b.seqs * c.heads * ((rows + 127) / 128);
+  if (rows > 64 && tiles >= 128 && tiles < 1 << 22 && (int64_t)c.ctx * c.dim < 0x7fff0000) return {0, 4, 1, kWhole};
   AttnPlan p;
-  if (rows > 64 && (int64_t)c.ctx * c.dim < 0x7fff0000 && (int64_t)b.seqs * c.heads * ((rows + 127) / 128) >= 128) return {0, 1, 0x40000000};
   p.rt = rows <= 16 ? 1 : 2;
   const int64_t groups = (int64_t)b.seqs * c.heads * ((rows + 16 * p.rt - 1) / (16 * p.rt));
   const int len = b.max_len < c.ctx ? (b.max_len > 0 ? b.max_len : 1) : c.ctx;
-  const int64_t want = groups >= 1024 ? 1 : (1024 + groups - 1) / groups;                // workgroups of four waves, four per CU
+  if (groups >= 1024 || len <= 128) return {p.rt, 4, 1, kWhole};                         // four workgroups of four waves per CU
+  if (len <= 1024) return {p.rt, 8, 1, kWhole};
+  const int64_t want = (1024 + groups - 1) / groups;
   const int most = (len + 127) / 128;                                                    // a wave's turn is 32 positions
   const int n = (int)(want < most ? want : most);
+  p.waves = 4;
   p.chunk = ((len + n - 1) / n + 127) / 128 * 128;
   p.nsplit = (len + p.chunk - 1) / p.chunk;
   return p;
 }
 
 template <typename T, int HD, int RT>
-int start_attention(const AttnArgs& a, hipStream_t s) {
-  const int64_t rows = (int64_t)(a.s.b.max_new > 0 ? a.s.b.max_new : 1) * a.per;
-  const int64_t blocks = (rows + 16 * RT - 1) / (16 * RT);
-  hipLaunchKernelGGL((kv8_attn_rows_kernel<T, HD, RT>), dim3((unsigned)(blocks * a.nsplit), a.s.c.heads, a.s.b.seqs), dim3(256), 0, s, a);
+int start_attention(const AttnArgs& a, int waves, hipStream_t s) {
+  const int64_t rows = (int64_t)most_new(a.s.b) * a.per;
+  const dim3 grid((unsigned)((rows + 16 * RT - 1) / (16 * RT) * a.nsplit), a.s.c.heads, a.s.b.seqs);
+  if constexpr (sizeof(T) == 2 || RT == 1) {
+    if (waves == 8) {
+      hipLaunchKernelGGL((kv8_attn_rows_kernel<T, HD, RT, 8>), grid, dim3(512), 0, s, a);
+      WJ_LAUNCH_CHECK();
+      return WJ_OK;
+    }
+  }
+  hipLaunchKernelGGL((kv8_attn_rows_kernel<T, HD, RT, 4>), grid, dim3(256), 0, s, a);
   WJ_LAUNCH_CHECK();
   if (a.nsplit > 1) {
-    const int64_t groups = ((int64_t)(a.s.b.max_new > 0 ? a.s.b.max_new : 1) * a.n_heads + 15) / 16;
+    const int64_t groups = ((int64_t)most_new(a.s.b) * a.n_heads + 15) / 16;
     hipLaunchKernelGGL((kv8_attn_join_kernel<T, HD>), dim3((unsigned)groups, a.s.b.seqs), dim3(256), 0, s, a, 16 * RT);
     WJ_LAUNCH_CHECK();
   }
@@ -761,7 +776,7 @@ int start_tile(const AttnArgs& a, hipStream_t s) {
     WJ_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kv8_attn_tile_kernel<T, HD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     once.done();
   }
-  const int64_t rows = (int64_t)a.s.b.max_new * a.per, blocks = (rows + 127) / 128, groups = (int64_t)a.s.b.seqs * a.s.c.heads;
+  const int64_t rows = (int64_t)most_new(a.s.b) * a.per, blocks = (rows + 127) / 128, groups = (int64_t)a.s.b.seqs * a.s.c.heads;
   hipLaunchKernelGGL((kv8_attn_tile_kernel<T, HD>), dim3((unsigned)((groups + 7) / 8 * 8 * blocks)), dim3(256), lds, s, a, (int)blocks);
   WJ_LAUNCH_CHECK();
   return WJ_OK;
@@ -771,7 +786,7 @@ int pick_rows(const AttnArgs& a, const AttnPlan& p, hipStream_t s) {
   if (p.rt == 0) {
     if constexpr (sizeof(T) == 2) return start_tile<T, HD>(a, s);
   }
-  return p.rt == 1 ? start_attention<T, HD, 1>(a, s) : start_attention<T, HD, 2>(a, s);
+  return p.rt == 1 ? start_attention<T, HD, 1>(a, p.waves, s) : start_attention<T, HD, 2>(a, p.waves, s);
 }
 template <int HD>
 int pick_type(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t s) {
@@ -792,7 +807,7 @@ int wj_kv8_write(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, in
   WJ_REQUIRE(ldk >= 0 && ldv >= 0, "wj_kv8_write: negative stride");
   DeviceScope dev;
   WJ_HIP(dev.enter(ctx->device));
-  const int64_t pairs = (int64_t)(batch->max_new > 0 ? batch->max_new : 1) * cache->heads;
+  const int64_t pairs = (int64_t)most_new(*batch) * cache->heads;
   return launch_write(cache, batch, dtype, k_dev, ldk, v_dev, ldv, pairs, ctx->pick(stream));
 }
 
@@ -805,7 +820,7 @@ int wj_kv8_read(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int
   WJ_REQUIRE(batch->rows == 1 || (ldk >= cache->heads * cache->dim && ldv >= cache->heads * cache->dim), "wj_kv8_read: output rows overlap");
   DeviceScope dev;
   WJ_HIP(dev.enter(ctx->device));
-  const int64_t pairs = (int64_t)(batch->max_new > 0 ? batch->max_new : 1) * cache->heads;
+  const int64_t pairs = (int64_t)most_new(*batch) * cache->heads;
   return launch_read(cache, batch, dtype, k_dev, ldk, v_dev, ldv, pairs, ctx->pick(stream));
 }
 

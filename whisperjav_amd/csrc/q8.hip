@@ -58,8 +58,9 @@ template <int WPR> __device__ __forceinline__ float row_max(float v, float* part
 template <RowMode MODE, int WPR, typename X, typename D>
 __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void q8_rows_kernel(const RowArgs a) {
   __shared__ float part[2][WPR];
-  const int64_t r = WPR == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
-  if (r >= a.rows) return;                     // WPR == 1 only, where no barrier follows
+  const int64_t group = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const int64_t r = WPR == 1 ? group * 4 + (threadIdx.x >> 6) : group;
+  if (r >= a.rows) return;                     // whole workgroups, or whole waves of one without barriers
   const int tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
   const X* x = reinterpret_cast<const X*>(a.x) + r * a.ldx;
   const int whole = a.cols & ~7;               // columns in whole groups of 8
@@ -674,7 +675,8 @@ __global__ __launch_bounds__(256) void q8_gemm_any_kernel(const GemmQ8Args g, in
 template <RowMode MODE, int WPR, typename X, typename D>
 int start_rows(const RowArgs& a, hipStream_t s) {
   const int64_t groups = WPR == 1 ? (a.rows + 3) / 4 : a.rows;
-  hipLaunchKernelGGL((q8_rows_kernel<MODE, WPR, X, D>), dim3((unsigned)groups), dim3(WPR == 1 ? 256 : WPR * 64), 0, s, a);
+  const int64_t nx = groups < (1 << 21) ? groups : 1 << 21;          // a grid's axis holds 2^32 threads
+  hipLaunchKernelGGL((q8_rows_kernel<MODE, WPR, X, D>), dim3((unsigned)nx, (unsigned)((groups + nx - 1) / nx)), dim3(WPR == 1 ? 256 : WPR * 64), 0, s, a);
   WJ_LAUNCH_CHECK();
   return WJ_OK;
 }

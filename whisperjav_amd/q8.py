@@ -5,8 +5,8 @@ rows, ``gemm`` multiplies them with weights held the same way (a scale per token
 like that, ``kv_write`` / ``kv_read`` / ``kv_attention`` fill, read back and attend to it.
 
 Every function launches on torch's current stream of the tensors' device and returns at once; outputs come from torch's allocator.  The
-calls may be captured into a ``torch.cuda.graph``.  Arguments are checked on the host (``ValueError``); the library's own refusals raise
-``hipbind.WjError``.  There is no CPU path.
+calls may be captured into a ``torch.cuda.graph``.  They serve inference and refuse tensors that want a gradient.  Arguments are checked
+on the host (``ValueError``); the library's own refusals raise ``hipbind.WjError``.  There is no CPU path.
 
 A decoder layer::
 
@@ -48,7 +48,11 @@ def _launch(index: int):
     """(library, context handle, stream) for tensors on GPU ``index``.  The calls of a decode step are bound by the host: the raw stream
     handle costs 0.1 us where a ``torch.cuda.Stream`` object costs 2."""
     stream = torch._C._cuda_getCurrentRawStream(index)
-    return hipbind.lib(), hipbind.context(index).handle, stream or _STREAM_DEFAULT
+    ctx = hipbind._contexts.get(index)
+    if ctx is None:
+        with torch.cuda.device(index):          # wj_init makes its GPU the thread's current one: put it back
+            ctx = hipbind.context(index)
+    return hipbind.lib(), ctx.handle, stream or _STREAM_DEFAULT
 
 
 def _fail(name: str, rc: int) -> None:
@@ -67,6 +71,8 @@ def _float_rows(t: torch.Tensor, what: str, index: Optional[int] = None, rows: i
         raise ValueError(f"{what}: on {t.device}, expected {'a GPU' if index is None else f'cuda:{index}'}")
     if t.stride(1) != 1 and shape[1] > 1:
         raise ValueError(f"{what}: the elements of a row must be contiguous (stride {t.stride(1)})")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: requires a gradient; these operators have none (torch.no_grad() to go on)")
     return code
 
 
@@ -96,8 +102,8 @@ def _output(t: torch.Tensor, what: str) -> None:
 def _new_codes(rows: int, cols: int, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows that start at multiples of 16 bytes, as the product's fast kernels want them."""
     pad = (cols + 15) & ~15
-    codes = torch.empty((rows, pad), dtype=torch.int8, device=device)
-    return codes if pad == cols else codes[:, :cols], torch.empty((rows,), dtype=torch.float32, device=device)
+    codes = torch.empty(rows, pad, dtype=torch.int8, device=device)
+    return codes if pad == cols else codes[:, :cols], torch.empty(rows, dtype=torch.float32, device=device)
 
 
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, delta: Optional[torch.Tensor] = None,
@@ -154,7 +160,7 @@ def dequantize(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = to
     if dtype not in _TYPE:
         raise ValueError(f"dtype: float32, float16 or bfloat16 expected, got {dtype}")
     rows, cols = codes.shape
-    out = torch.empty((rows, cols), dtype=dtype, device=codes.device)
+    out = torch.empty(rows, cols, dtype=dtype, device=codes.device)
     lib, ctx, stream = _launch(index)
     rc = lib.wj_q8_dequantize(ctx, codes.data_ptr(), codes.stride(0), scale.data_ptr(), _TYPE[dtype], out.data_ptr(), cols, rows, cols, stream)
     if rc:
@@ -179,13 +185,13 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
         dt = _TYPE.get(dtype)
         if dt is None:
             raise ValueError(f"dtype: float32, float16 or bfloat16 expected, got {dtype}")
-        out = torch.empty((m, n), dtype=dtype, device=a.device)
+        out = torch.empty(m, n, dtype=dtype, device=a.device)
     else:
         dt = _float_rows(out, "out", index, m, n)
         _output(out, "out")
     lib, ctx, stream = _launch(index)
     need = lib.wj_q8_gemm_workspace(ctx, m, n, k)
-    work = torch.empty((need,), dtype=torch.uint8, device=a.device) if need else None      # freed in stream order by torch's allocator
+    work = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None      # freed in stream order by torch's allocator
     rc = lib.wj_q8_gemm(ctx, a.data_ptr(), a.stride(0), a_scale.data_ptr(), w.data_ptr(), w.stride(0), w_scale.data_ptr(),
                         bias.data_ptr() if bias is not None else None, dt, out.data_ptr(), out.stride(0), m, n, k,
                         work.data_ptr() if need else None, need, stream)
@@ -273,6 +279,8 @@ def _head_rows(t: torch.Tensor, what: str, cache: Kv8C, index: int, heads: Optio
         raise ValueError(f"{what}: float32, float16 or bfloat16 expected, got {t.dtype}")
     if t.get_device() != index:
         raise ValueError(f"{what}: on {t.device}, expected cuda:{index}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: requires a gradient; these operators have none (torch.no_grad() to go on)")
     stride = t.stride()
     if stride[2] != 1 or (shape[1] > 1 and stride[1] != cache.dim):
         raise ValueError(f"{what}: the heads of a row must lie one after the other, their elements too (strides {stride})")
@@ -301,8 +309,8 @@ def kv_read(cache: KV8Cache, batch: Batch, rows: int, dtype: torch.dtype = torch
         raise ValueError(f"rows: {rows}")
     b = _batch(batch, rows, index)
     heads, dim, device = c.heads, c.dim, cache.k.device
-    k = torch.empty((rows, heads, dim), dtype=dtype, device=device)
-    v = torch.empty((rows, heads, dim), dtype=dtype, device=device)
+    k = torch.empty(rows, heads, dim, dtype=dtype, device=device)
+    v = torch.empty(rows, heads, dim, dtype=dtype, device=device)
     lib, ctx, stream = _launch(index)
     rc = lib.wj_kv8_read(ctx, C.byref(c), C.byref(b), _TYPE[dtype], k.data_ptr(), heads * dim, v.data_ptr(), heads * dim, stream)
     if rc:
@@ -319,14 +327,14 @@ def kv_attention(q: torch.Tensor, cache: KV8Cache, batch: Batch, *, causal: bool
     dt = _head_rows(q, "q", c, index)
     rows, heads, dim = q.shape
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty(rows, heads, dim, dtype=q.dtype, device=q.device)
     elif _head_rows(out, "out", c, index, heads) != dt or out.shape[0] != rows or (rows > 1 and out.stride(0) < heads * dim):
         raise ValueError(f"out: {list(q.shape)} in {q.dtype} expected, rows apart, got {list(out.shape)} in {out.dtype}")
     b = _batch(batch, rows, index)
     lib, ctx, stream = _launch(index)
     cp, bp = C.byref(c), C.byref(b)
     need = lib.wj_kv8_attention_workspace(ctx, cp, bp, heads)
-    work = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None      # freed in stream order by torch's allocator
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None      # freed in stream order by torch's allocator
     rc = lib.wj_kv8_attention(ctx, cp, bp, dt, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), heads, dim ** -0.5 if scale is None else scale,
                               1 if causal else 0, work.data_ptr() if need else None, need, stream)
     if rc:
