@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, T* __res
 // Attention over the cache.
 //
 // Per key / value head the rows of a sequence are its (new row, query head of the group) pairs, r = t * per + g; a workgroup takes
-// 16 RT of them and a range of positions, its waves (four, or eight) take 32 positions at a time in turn.  Codes go from memory straight into the
+// 16 RT of them and a range of positions, its waves (four, or eight for 16 rows) take 32 positions at a time in turn.  Codes go from memory straight into the
 // operands of the matrix cores: S^T = K Q^T per 16 positions, the positions of two such products permuted so that the weights leave the
 // first product in the order the second one, O^T += V^T P^T, wants them.  An int8 code is exact in float16 (byte | 0x6400 is 1024 + byte,
 // minus 1152), so the products lose nothing of the cache; the query is carried in units of a power of two that bounds its row, exact for
@@ -725,7 +725,14 @@ int launch_read(const wj_kv8* c, const wj_kv8_batch* b, int dtype, void* k, int6
   return start_read<bf16_t, 64>(c, b, k, ldk, v, ldv, pairs, s);
 }
 
-// Rows and waves per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).
+// Rows and waves per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).  Measured on the MI355X (us a
+// call in a graph; float16, 8 heads of 128 and 1 .. 4 queries each unless said otherwise):
+//   16 rows, up to 1024 positions, four / eight waves: 16 sequences x 500 9.1 / 8.2, 16 x 1000 13.5 / 11.9, 64 x 500 13.2 / 15.8, 200 x 500
+//     36 / 49: eight where there are fewer than 256 workgroups (four parts and a join: 9.8 and 12.5, and 3.5 us more for the host);
+//   16 rows, more positions, one / two / four / eight parts: 1 x 4000 33 / 22 / 16 / 13, 16 x 4000 40 / 28 / 27 / 30, 64 x 1500 33 / 36 / 37 / 39,
+//     16 x 20 heads of 64 x 4000 45 / 37 / 34 / 37;
+//   32 rows: 1 x 1000 16 / 14 / 12 / 12, 16 x 1000 18 / 17 / 19 / 25, 16 x 4000 53 / 35 / 34 / 40, 64 x 1000 29 / 39 / 49 / 72, 1 x 500 10.6 / 11 / 10.3.
+// So parts make up to 512 workgroups, of 256 positions or more, at most 8.
 struct AttnPlan { int rt, waves, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel (16-bit types; float32 rows take two blocks)
 constexpr int kWhole = 0x40000000;
 AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
@@ -733,26 +740,23 @@ AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
   const int64_t rows = (int64_t)most_new(b) * per;
   const int64_t tiles = (int64_t)b.seqs * c.heads * ((rows + 127) / 128);
   if (rows > 64 && tiles >= 128 && tiles < 1 << 22 && (int64_t)c.ctx * c.dim < 0x7fff0000) return {0, 4, 1, kWhole};
-  AttnPlan p;
-  p.rt = rows <= 16 ? 1 : 2;
-  const int64_t groups = (int64_t)b.seqs * c.heads * ((rows + 16 * p.rt - 1) / (16 * p.rt));
+  const int rt = rows <= 16 ? 1 : 2;
+  const int64_t groups = (int64_t)b.seqs * c.heads * ((rows + 16 * rt - 1) / (16 * rt));
   const int len = b.max_len < c.ctx ? (b.max_len > 0 ? b.max_len : 1) : c.ctx;
-  if (groups >= 1024 || len <= 128) return {p.rt, 4, 1, kWhole};                         // four workgroups of four waves per CU
-  if (len <= 1024) return {p.rt, 8, 1, kWhole};
-  const int64_t want = (1024 + groups - 1) / groups;
-  const int most = (len + 127) / 128;                                                    // a wave's turn is 32 positions
-  const int n = (int)(want < most ? want : most);
-  p.waves = 4;
-  p.chunk = ((len + n - 1) / n + 127) / 128 * 128;
-  p.nsplit = (len + p.chunk - 1) / p.chunk;
-  return p;
+  if (rt == 1 && len <= 1024) return {1, len > 128 && groups < 256 ? 8 : 4, 1, kWhole};
+  int64_t parts = (512 + groups - 1) / groups;
+  parts = parts > 8 ? 8 : parts;
+  parts = parts > (len + 255) / 256 ? (len + 255) / 256 : parts;
+  if (parts <= 1 || (rt == 2 && len <= 512)) return {rt, 4, 1, kWhole};
+  const int chunk = (int)(((len + parts - 1) / parts + 127) / 128 * 128);
+  return {rt, 4, (len + chunk - 1) / chunk, chunk};
 }
 
 template <typename T, int HD, int RT>
 int start_attention(const AttnArgs& a, int waves, hipStream_t s) {
   const int64_t rows = (int64_t)most_new(a.s.b) * a.per;
   const dim3 grid((unsigned)((rows + 16 * RT - 1) / (16 * RT) * a.nsplit), a.s.c.heads, a.s.b.seqs);
-  if constexpr (sizeof(T) == 2 || RT == 1) {
+  if constexpr (RT == 1) {
     if (waves == 8) {
       hipLaunchKernelGGL((kv8_attn_rows_kernel<T, HD, RT, 8>), grid, dim3(512), 0, s, a);
       WJ_LAUNCH_CHECK();
