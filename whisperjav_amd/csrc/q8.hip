@@ -63,94 +63,114 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void q8_rows_kernel(cons
   if (r >= a.rows) return;                     // whole workgroups, or whole waves of one without barriers
   const int tid = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
   const X* x = reinterpret_cast<const X*>(a.x) + r * a.ldx;
-  const int whole = a.cols & ~7;               // columns in whole groups of 8
-  float v[kSteps][8];
+  const int whole = a.cols & ~7;               // columns in whole groups of 8; the one group after them goes element by element
+  const bool tail = a.cols & 7;
+  auto col = [&](int s) { return (s * WPR * 64 + tid) * 8; };
+  float v[kSteps][8], ss = 0.f, top = 0.f;
   if constexpr (MODE == ROW_SWIGLU) {
-    // the group's 8 gate columns lie together when groups do not straddle blocks
-    const bool wide = a.block % 8 == 0 || a.block == a.cols;
+    // a group's 8 gate columns lie together when groups do not straddle blocks
+    if (a.block % 8 == 0 || a.block == a.cols) {
+      Raw8<X> gate[kSteps] = {}, up[kSteps] = {};
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int c = (s * WPR * 64 + tid) * 8;
-      if (c < whole && wide) {
-        const X* g = x + (int64_t)(c / a.block) * 2 * a.block + c % a.block;
-        float gate[8], up[8];
-        const Raw8<X> rg = ld_raw8(g), ru = ld_raw8(g + a.block);
-        widen8(rg, gate); widen8(ru, up);
+      for (int s = 0; s < kSteps; ++s) {
+        const int c = col(s);
+        if (c < whole) {
+          const X* g = x + (int64_t)(c / a.block) * 2 * a.block + c % a.block;
+          gate[s] = ld_raw8(g);
+          up[s] = ld_raw8(g + a.block);
+        }
+      }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[s][e] = silu_mul(gate[e], up[e]);
-      } else {
+      for (int s = 0; s < kSteps; ++s) {
+        float g[8], u[8];
+        widen8(gate[s], g); widen8(up[s], u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[s][e] = silu_mul(g[e], u[e]);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
+          const int c = col(s) + e;
           v[s][e] = 0.f;
-          if (c + e < a.cols) {
-            const X* g = x + (int64_t)((c + e) / a.block) * 2 * a.block + (c + e) % a.block;
+          if (c < whole) {
+            const X* g = x + (int64_t)(c / a.block) * 2 * a.block + c % a.block;
             v[s][e] = silu_mul(Elem<X>::ld(g), Elem<X>::ld(g + a.block));
           }
         }
-      }
     }
+    if (tail)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (col(s) == whole)
+#pragma unroll
+          for (int e = 0; e < 7; ++e) {
+            const int c = whole + e;
+            const X* g = x + (int64_t)(c / a.block) * 2 * a.block + c % a.block;
+            if (c < a.cols) v[s][e] = silu_mul(Elem<X>::ld(g), Elem<X>::ld(g + a.block));
+          }
   } else {
+    // everything the row needs is requested before the first value is used
+    constexpr bool HAS_DELTA = !std::is_same<D, NoType>::value;
+    typedef typename std::conditional<HAS_DELTA, D, f16_t>::type DT;
+    const DT* d = reinterpret_cast<const DT*>(a.delta) + r * a.ldd;
+    Raw8<X> rx[kSteps] = {};
+    Raw8<DT> rd[kSteps] = {};
+    Raw8<float> rw[kSteps] = {};
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int c = (s * WPR * 64 + tid) * 8;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[s][e] = 0.f;
-      if (c < whole) widen8(ld_raw8(x + c), v[s]);
-      else
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (c + e < a.cols) v[s][e] = Elem<X>::ld(x + c + e);
+      const int c = col(s);
+      if (c < whole) {
+        rx[s] = ld_raw8(x + c);
+        if constexpr (HAS_DELTA) rd[s] = ld_raw8(d + c);
+        if constexpr (MODE == ROW_NORM) rw[s] = ld_raw8(a.w + c);
+      }
     }
-  }
-  float ss = 0.f, top = 0.f;
-  if constexpr (MODE == ROW_NORM) {
-    if constexpr (!std::is_same<D, NoType>::value) {
-      const D* d = reinterpret_cast<const D*>(a.delta) + r * a.ldd;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int c = (s * WPR * 64 + tid) * 8;
-        if (c < whole) {
-          float t[8];
-          widen8(ld_raw8(d + c), t);
+    for (int s = 0; s < kSteps; ++s) {
+      widen8(rx[s], v[s]);
+      if constexpr (HAS_DELTA) {
+        float t[8];
+        widen8(rd[s], t);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[s][e] += t[e];
-        } else {
+        for (int e = 0; e < 8; ++e) v[s][e] += t[e];
+      }
+    }
+    if (tail)
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        if (col(s) == whole)
 #pragma unroll
           for (int e = 0; e < 7; ++e)
-            if (c + e < a.cols) v[s][e] += Elem<D>::ld(d + c + e);
+            if (whole + e < a.cols) {
+              v[s][e] = Elem<X>::ld(x + whole + e);
+              if constexpr (HAS_DELTA) v[s][e] += Elem<D>::ld(d + whole + e);
+              if constexpr (MODE == ROW_NORM) rw[s].w[e] = __float_as_uint(a.w[whole + e]);
+            }
+    if constexpr (MODE == ROW_NORM) {
+      if (a.resid) {
+        X* o = reinterpret_cast<X*>(a.resid) + r * a.ldr;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const int c = col(s);
+          if (c < whole) st8<X>(o + c, v[s]);
+          else if (c == whole)
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+              if (c + e < a.cols) o[c + e] = to_T<X>(v[s][e]);
         }
       }
-    }
-    if (a.resid) {
-      X* o = reinterpret_cast<X*>(a.resid) + r * a.ldr;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int c = (s * WPR * 64 + tid) * 8;
-        if (c < whole) st8<X>(o + c, v[s]);
-        else
+      for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-          for (int e = 0; e < 7; ++e)
-            if (c + e < a.cols) o[c + e] = to_T<X>(v[s][e]);
-      }
-    }
+        for (int e = 0; e < 8; ++e) ss += v[s][e] * v[s][e];
+      const float scale = rsqrtf(row_sum<WPR>(ss, part[0]) / (float)a.cols + a.eps);
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
+      for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += v[s][e] * v[s][e];
-    const float scale = rsqrtf(row_sum<WPR>(ss, part[0]) / (float)a.cols + a.eps);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const int c = (s * WPR * 64 + tid) * 8;
-      if (c < whole) {
-        float w[8];
-        widen8(ld_raw8(a.w + c), w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[s][e] = v[s][e] * scale * w[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (c + e < a.cols) v[s][e] = v[s][e] * scale * a.w[c + e];
-      }
+        for (int e = 0; e < 8; ++e)            // past the row: zeros, unless the row itself is not finite
+          v[s][e] = v[s][e] * scale * __uint_as_float(rw[s].w[e]);
     }
   }
 #pragma unroll
@@ -161,12 +181,12 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void q8_rows_kernel(cons
   int8_t* o = a.codes + r * a.ldc;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
-    const int c = (s * WPR * 64 + tid) * 8;
+    const int c = col(s);
     if (c < whole) {
       const uint32_t w[2] = {pack4(q.code(v[s][0]), q.code(v[s][1]), q.code(v[s][2]), q.code(v[s][3])),
                              pack4(q.code(v[s][4]), q.code(v[s][5]), q.code(v[s][6]), q.code(v[s][7]))};
       __builtin_memcpy(o + c, w, 8);
-    } else {
+    } else if (c == whole) {
 #pragma unroll
       for (int e = 0; e < 7; ++e)
         if (c + e < a.cols) o[c + e] = (int8_t)q.code(v[s][e]);
@@ -683,7 +703,7 @@ int start_rows(const RowArgs& a, hipStream_t s) {
 template <RowMode MODE, typename X, typename D>
 int pick_rows(const RowArgs& a, hipStream_t s) {
   if (a.cols <= 2048 && a.rows >= 2048) return start_rows<MODE, 1, X, D>(a, s);
-  if (a.cols <= 8192) return start_rows<MODE, 4, X, D>(a, s);
+  if (a.cols <= 2048 || (a.cols <= 8192 && a.rows > 256)) return start_rows<MODE, 4, X, D>(a, s);
   return start_rows<MODE, 16, X, D>(a, s);
 }
 template <RowMode MODE, typename X>
