@@ -11,9 +11,10 @@ namespace {
 // --------------------------------------------------------------------------------------------
 // Rows.  WPR waves hold one row in registers, 8 consecutive columns per lane and step (at most 4 steps): one read of the inputs, one
 // write of the outputs, the sum of squares and the maximum over lanes by shuffles (and over waves through LDS).  Bound by memory: the
-// norm of 2048 float32 + float16 columns moves 11 bytes per element.  Rows of any stride and base are read with wide loads (gfx950
-// serves unaligned ones).  One wave per row when there are rows to fill the chip with (no barrier between the passes); else 4 or 16, which
-// shortens the chain of loads of a call that is bound by latency.
+// norm of 16384 x 2048 float32 + float16 moves 11 bytes per element (369 MB with the weight) in 73 us, 5.0 TB/s, back to back in cold caches;
+// one row takes 4.3 us, which is the launch and two round trips.  Everything a row needs is requested before its first value is used.  Rows of any stride and base are read with wide loads (gfx950
+// serves unaligned ones).  One wave per row when there are rows to fill the chip with (no barrier between the passes); else 4, which
+// shortens the chain of loads of a call that is bound by latency (see pick_rows).
 // --------------------------------------------------------------------------------------------
 struct RowArgs {
   const void* x; int64_t ldx;
@@ -199,7 +200,8 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void q8_rows_kernel(cons
   if (tid == 0) a.scale[r] = q.scale;
 }
 
-// Read-back: a workgroup takes whole rows' groups of 8 columns in turn, one wide load and store each.
+// Read-back: a workgroup takes whole rows' groups of 8 columns in turn, one wide load and store each.  16383 x 2040 to bfloat16 (100 MB): 15.4 us, 6.5
+// TB/s, the codes partly from the caches they were just written to.
 template <typename T>
 __global__ __launch_bounds__(256) void q8_dequantize_kernel(const int8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scale,
                                                             T* __restrict__ out, int64_t ldo, int64_t rows, int cols) {
@@ -369,6 +371,7 @@ __device__ __forceinline__ void tile_of(int lin, int nx, int ny, int* tx, int* t
 // WAR: the other buffer held pair p - 1, read last in group 1's MEM(2p - 1), retired before B(4p - 1); MEM(2p) starts after it.
 // RAW: both groups have waited for pair p + 1 by B(4p + 3); it is first read after that.
 // 128-byte LDS rows, 16-byte piece c of row r in place c ^ (r & 7).
+// Bound by the matrix pipe: 16384 x 12288 x 2048 in 395 us, 2.09 POP/s.
 template <typename T, bool PAST>
 __global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, int nx, int ny) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [buffer][A | W][256][128]
@@ -458,10 +461,11 @@ __global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, in
 // BM x 128 tile, k steps of 128 codes, a ring of 3 buffers with 2 steps requested ahead (BM = 64: two workgroups per CU).  Eight waves: (2 x 2, BM / 2 x 64 each) twice,
 // each four taking one half of every step's codes, so that the two waves of a SIMD overlap one's LDS reads with the other's products; the
 // two halves' sums meet in LDS at the end, each four finishing half of the rows.  For calls with too few 256-tiles to fill the chip;
-// ksplit > 1: slices of k on the grid's second axis write raw sums, joined by q8_gemm_join_kernel.
+// ksplit > 1: slices of k on the grid's second axis write raw sums, joined by q8_gemm_join_kernel.  Bound by LDS traffic (DMA in, fragments out):
+// 240 x 12288 x 2048 in 14 us, 0.38 us per step of a 64-row tile (0.23 with the DMA taken away).
 template <typename T, int BM>
 __global__ __launch_bounds__(512) void q8_gemm_tile_kernel(const GemmQ8Args g, int nx, int ny) {
-  extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [stage][A: 64 | W: 128][128]
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [stage][A: BM | W: 128][128]
   constexpr int NS = 3, STAGE = (BM + 128) * 128, RI = BM / 32, QA = BM / 64;      // 16-row blocks and requests of a wave
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -597,7 +601,8 @@ __global__ __launch_bounds__(256) void q8_gemm_join_kernel(const GemmQ8Args g) {
 }
 
 // Few rows (at most 16 MT): bound by the weights' bytes.  A workgroup owns 16 output columns, its 8 waves split k, the weights go straight
-// from memory into the operands (every byte once), the 8 partial tiles meet in LDS.
+// from memory into the operands (every byte once), the 8 partial tiles meet in LDS.  1 x 4096 x 2048 in 3.9 us: the launch and one round trip;
+// 8 steps ahead instead of 4 take 4.6 (requests past a wave's share of k).
 template <typename T, int MT>
 __global__ __launch_bounds__(512) void q8_gemm_rows_kernel(const GemmQ8Args g) {
   __shared__ __attribute__((aligned(16))) int red[8 * MT * 256];
@@ -657,7 +662,7 @@ __global__ __launch_bounds__(512) void q8_gemm_rows_kernel(const GemmQ8Args g) {
   }
 }
 
-// Any base, stride and size: 64 x 64 tile, k step 64, operands gathered byte by byte into LDS, 4 waves of 16 rows x 64 columns.
+// Any base, stride and size (the caller's own layout, not a path to be fast on: 16384 x 12288 x 2048 takes 21 ms): 64 x 64 tile, k step 64, operands gathered byte by byte into LDS, 4 waves of 16 rows x 64 columns.
 __global__ __launch_bounds__(256) void q8_gemm_any_kernel(const GemmQ8Args g, int dtype) {
   __shared__ __attribute__((aligned(16))) int8_t la[64 * 80], lw[64 * 80];      // rows 80 bytes apart: 16-byte reads, few bank conflicts
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -704,10 +709,15 @@ int start_rows(const RowArgs& a, hipStream_t s) {
   WJ_LAUNCH_CHECK();
   return WJ_OK;
 }
+// Waves per row, us per call in a graph, norm (float32 + float16) / bfloat16 quantisation / float16 SwiGLU:
+//   1 wave against 4: 24 x 2048 4.2, 3.3, 5.2 / 4.0, 3.1, 3.7; 512 x 2048 5.1, 3.5, 5.5 / 5.0, 3.5, 4.4; 1024 x 2048 6.4, 3.7, 5.7 / 7.1, 4.5, 6.1;
+//     1024 x 512 4.1, 3.1, 3.8 / 5.3, 4.1, 5.3; 16384 x 2048 56, 18, 41 / 60, 29, 47;
+//   4 waves against 16: 1 x 8192 4.3, 3.2, 5.1 / 5.2, 3.7, 5.0; 256 x 6144 5.7, 3.6, 5.2 / 6.5, 4.3, 5.7; 2048 x 4096 17, 7, 14 / 35, 16, 30.
+// So 16 are for rows that 4 cannot hold, beyond 8192 columns.
 template <RowMode MODE, typename X, typename D>
 int pick_rows(const RowArgs& a, hipStream_t s) {
-  if (a.cols <= 2048 && a.rows >= 2048) return start_rows<MODE, 1, X, D>(a, s);
-  if (a.cols <= 2048 || (a.cols <= 8192 && a.rows > 256)) return start_rows<MODE, 4, X, D>(a, s);
+  if (a.cols <= 2048 && a.rows >= 1024) return start_rows<MODE, 1, X, D>(a, s);
+  if (a.cols <= 8192) return start_rows<MODE, 4, X, D>(a, s);
   return start_rows<MODE, 16, X, D>(a, s);
 }
 template <RowMode MODE, typename X>
