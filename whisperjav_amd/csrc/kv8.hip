@@ -30,8 +30,8 @@ __device__ __forceinline__ Span span_of(const Kv8Args& a, int b) {
 }
 
 // Writing: HD / 8 lanes hold one head's row of K and of V, 8 elements each, read and written with one wide access per lane and tensor; the
-// maximum goes over the lanes by exchanges.  Bound by memory: a 16-bit row of 128 moves 256 + 128 + 4 bytes.  A workgroup takes (row, head)
-// pairs of one sequence in turn.
+// maximum goes over the lanes by exchanges.  Bound by memory: a 16-bit row of 128 moves 256 + 128 + 4 bytes; 20 k rows of 8 heads of K and V are
+// written in 31 us (4.1 TB/s) and read back in 23 (5.5).  A workgroup takes (row, head) pairs of one sequence in turn.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv8_write_kernel(const Kv8Args a, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v,
                                                         int64_t ldv) {
@@ -99,8 +99,9 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, T* __res
 // 16-bit types, as a high and a low half (22 bits) for float32.
 //
 // Weights: with x = scale * log2(e) * ks * (q . k), the numerator of a position is 2^x vs, and 16 bits must hold it whatever the
-// scales are.  So the running reference of a row is M = max(x + exponent of vs), numerators are 2^(x - M) vs (at most 2^4, the slack), the
-// denominator sums 2^(x - M) in float32.  M moves only when it would be exceeded by 2^4.  A numerator goes into the product as one half
+// scales are.  So the running reference of a row is M = max(x + exponent of vs) - 11, numerators are 2^(x - M) vs (at most 2^15), the
+// denominator sums 2^(x - M) in float32.  M moves only when the largest numerator would pass 2^15.  The smallest step of a half, 2^-24, is then
+// 2^-34 of the row's largest numerator or less: what a weight can lose for being small.  A numerator goes into the product as one half
 // for bfloat16 rows (2^-12 of a weight, an eighth of what rounding the output costs) and as a high and a low half (22 bits) for float16
 // and float32 rows: with one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 (512 sequences; 124 us either way, the
 // matrix pipe has room).
@@ -117,7 +118,7 @@ struct AttnArgs {
   float2* ml;                // ... and (M, denominator)
 };
 
-constexpr float kSlack = 4.f;
+constexpr float kRoom = 11.f, kSlack = 15.f;
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ uint32_t h2_less(uint32_t w) {      // two halves, 1152 taken off each
@@ -153,7 +154,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 }
 
 __device__ __forceinline__ float scale_exponent(float vs) {      // of a value scale, bounded so that 2^(x - M) and its sums stay in range
-  return vs == 0.f ? -100.f : fminf(fmaxf((float)__builtin_amdgcn_frexp_expf(vs), -100.f), 110.f);
+  return vs == 0.f ? -90.f : fminf(fmaxf((float)__builtin_amdgcn_frexp_expf(vs), -90.f), 110.f);
 }
 
 __device__ __forceinline__ int over_per(const AttnArgs& a, int r) { return a.per == 1 ? r : (int)__umulhi((uint32_t)r, a.per_inv); }
@@ -353,8 +354,8 @@ __global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv
         }
         top = quad_max(top);
         if (top > M[t] + kSlack) {
-          const float f = __builtin_amdgcn_exp2f(M[t] - top);      // the first time: 0 on zeros
-          M[t] = top;
+          const float f = __builtin_amdgcn_exp2f(M[t] - (top - kRoom));      // the first time: 0 on zeros
+          M[t] = top - kRoom;
           l[t] *= f;
 #pragma unroll
           for (int e = 0; e < NE; ++e)
@@ -586,8 +587,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
         }
         top = quad_max(top);
         if (top > M[t] + kSlack) {
-          const float f = __builtin_amdgcn_exp2f(M[t] - top);
-          M[t] = top;
+          const float f = __builtin_amdgcn_exp2f(M[t] - (top - kRoom));
+          M[t] = top - kRoom;
           l[t] *= f;
 #pragma unroll
           for (int e = 0; e < NE; ++e)
@@ -687,10 +688,11 @@ int check_kv8(const char* who, wj_ctx* ctx, const wj_kv8* c, const wj_kv8_batch*
   return WJ_OK;
 }
 
-// (row, head) pairs of a sequence over workgroups: at most 4 turns each while there are enough of them
+// (row, head) pairs of a sequence over workgroups, one turn each (four turns: 1500 x 20 heads of 64 6.7 us instead of 5.3, 32 x 640 x 8 heads of 128
+// 24.9 instead of 24.8; reading 4.9 / 3.9 and 22.8 / 21.6)
 dim3 pair_grid(int64_t pairs, int per, int seqs) {
-  const int64_t groups = (pairs + per - 1) / per, want = groups * seqs > 8192 ? (groups + 3) / 4 : groups;
-  return dim3((unsigned)(want < 65536 ? want : 65536), seqs);
+  const int64_t groups = (pairs + per - 1) / per;
+  return dim3((unsigned)(groups < 65536 ? groups : 65536), seqs);
 }
 template <typename T, int HD>
 int start_write(const wj_kv8* c, const wj_kv8_batch* b, const void* k, int64_t ldk, const void* v, int64_t ldv, int64_t pairs, hipStream_t s) {
@@ -733,13 +735,18 @@ int launch_read(const wj_kv8* c, const wj_kv8_batch* b, int dtype, void* k, int6
 //     16 x 20 heads of 64 x 4000 45 / 37 / 34 / 37;
 //   32 rows: 1 x 1000 16 / 14 / 12 / 12, 16 x 1000 18 / 17 / 19 / 25, 16 x 4000 53 / 35 / 34 / 40, 64 x 1000 29 / 39 / 49 / 72, 1 x 500 10.6 / 11 / 10.3.
 // So parts make up to 512 workgroups, of 256 positions or more, at most 8.
+// The 128-row kernel against 32 rows per workgroup, new rows x queries per head, positions: 16 x 100 x 1, 500 25.7 / 19.0; 8 x 128 x 2, 1500 63.5 / 40;
+//   32 x 33 x 2, 500 26.1 / 26.0; 32 x 100 x 1, 500 and 1500 28.0 / 32.3 and 66 / 69; 4 x 500 x 2, 500 24.5 / 29.5; 16 x 500 x 2, 500 45 / 101;
+//   of 64 dims 32 x 100 x 1, 500 and 1500 20.9 / 21.8 and 53 / 47: a CU holds two of its workgroups, so it is for calls of more than three blocks
+//   of 32 rows per CU; up to 64 rows a sequence its waves would stand half idle (16 x 64 rows 24.0 / 12.6, 32 x 64 25.2 / 19.1).
 struct AttnPlan { int rt, waves, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel (16-bit types; float32 rows take two blocks)
 constexpr int kWhole = 0x40000000;
 AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
   const int per = n_heads / c.heads;
   const int64_t rows = (int64_t)most_new(b) * per;
   const int64_t tiles = (int64_t)b.seqs * c.heads * ((rows + 127) / 128);
-  if (rows > 64 && tiles >= 128 && tiles < 1 << 22 && (int64_t)c.ctx * c.dim < 0x7fff0000) return {0, 4, 1, kWhole};
+  const int64_t blocks32 = (int64_t)b.seqs * c.heads * ((rows + 31) / 32);
+  if (rows > 64 && blocks32 > 768 && tiles < 1 << 22 && (int64_t)c.ctx * c.dim < 0x7fff0000) return {0, 4, 1, kWhole};
   const int rt = rows <= 16 ? 1 : 2;
   const int64_t groups = (int64_t)b.seqs * c.heads * ((rows + 16 * rt - 1) / (16 * rt));
   const int len = b.max_len < c.ctx ? (b.max_len > 0 ? b.max_len : 1) : c.ctx;
