@@ -100,6 +100,31 @@ def test_rows_that_are_empty_or_not_finite(q8, cols):
     assert bool(torch.isnan(values[2:]).all()) and bool(torch.isfinite(values[:2]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_ties_go_to_the_even_code(q8, dtype):
+    """127 x / max that lies half way between two codes, exactly: maxima whose 127th part is no float32"""
+    tops = torch.tensor([1 + i / 32 for i in range(32)], dtype=torch.float64)
+    parts = torch.tensor([1.0, -0.5, 0.5, -0.0, 1 / 256, 3 / 256], dtype=torch.float64)                 # of the maximum, exact in both types
+    x = (tops[:, None] * parts).to(dtype)
+    codes, scale = q8.quantize(x.cuda())
+    exact = 127 * x.double() / tops[:, None]                                                           # multiples of 127 / 256: exact
+    assert torch.equal(codes.cpu().double(), torch.round(exact) + 0.0)
+    assert torch.equal(scale.cpu(), (tops / 127).float())
+    k = x.repeat(1, 11)[:, :64].reshape(32, 1, 64).cuda()
+    cache = q8.KV8Cache.empty(1, 1, 32, 64)
+    q8.kv_write(cache, k, -k, make_batch(q8, [0], [0, 32], [32]))
+    want = torch.round(exact).repeat(1, 11)[:, :64]
+    assert torch.equal(cache.k[0, 0].cpu().double(), want + 0.0) and torch.equal(cache.v[0, 0].cpu().double(), 0.0 - want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_the_largest_values(q8, dtype):
+    x = torch.randn(3, 300, generator=rng(1)).double()
+    x = (x / x.abs().max() * torch.tensor([3.38e38, 2e30, 1e37], dtype=torch.float64)[:, None]).to(dtype)
+    codes, scale = q8.quantize(x.cuda())
+    check_rows(codes, scale, x, 0.0)
+
+
 @pytest.mark.parametrize("rows,cols,block", [(1, 16, 16), (3, 48, 16), (24, 6144, 16), (5, 640, 640), (2, 33, 33), (4, 96, 8), (3, 6, 2), (2, 10000, 16), (1, 32768, 32768)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_quantize_swiglu(q8, rows, cols, block, dtype):
@@ -297,7 +322,11 @@ def check_attention(got, q, values, slots, starts, lens, causal, scale, dtype):
     e = 2 * (dim + 16) * E * top.clamp_max(1e6) + (keys / 8 + 64) * E
     if dtype != torch.float32:
         e = e + 2.0 ** -10                                                                # a weight carried in 16 bits, and their sum
-    lim = e[..., None] * spread + (U[dtype] + E) * want.abs() + TINY[dtype]
+    # A numerator is carried in halves, whose step is 2^-24 at least: off by 2^-25, times a code of at most 128.  The largest numerator is kept
+    # above 2^10 = 2^11 * (its value scale / that scale's next power of two), so the denominator is above 2^10 / vs for some vs: per position
+    # the output is off by 2^-25 * 128 vs / 2^10 = 2^-35 * 128 vs, whatever the small weights are, and 64 vs < max |v| here.
+    floor = keys * 2.0 ** -34 * v.abs().amax()
+    lim = e[..., None] * spread + (U[dtype] + E) * want.abs() + TINY[dtype] + floor
     got = got.cpu().double()
     owned = torch.zeros(q.shape[0], dtype=torch.bool)
     for _, t, _ in ref.spans(starts, lens, q.shape[0]):
@@ -341,7 +370,7 @@ def test_attention(q8, layout, dim, heads, per, dtype, causal):
         assert bool((out[:, heads * per] == 0).all()) and bool((out[-1] == 0).all())
 
 
-@pytest.mark.parametrize("dim,heads,per", [(64, 4, 1), (64, 2, 3), (128, 3, 2), (128, 2, 4)])
+@pytest.mark.parametrize("dim,heads,per", [(64, 4, 1), (64, 2, 3), (128, 3, 2), (128, 2, 4), (64, 8, 1), (128, 8, 1), (64, 1, 16)])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("causal", [True, False])
 def test_attention_of_many_prompts(q8, dim, heads, per, dtype, causal):
@@ -413,6 +442,35 @@ def test_attention_of_a_row_that_is_not_finite(q8, new):
         sees = 100 - new + t >= 90
         assert bool(torch.isnan(got[t]).all()) == sees and bool(torch.isfinite(got[t]).all()) != sees
     assert bool(torch.isnan(got[new, 1]).all()) and bool(torch.isfinite(got[new, 0]).all()) and bool(torch.isfinite(got[new + 1:]).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_prompts_with_rows_that_are_not_finite_or_peaked(q8, dim, dtype):
+    """in the kernel for many rows: NaN stays with the rows that see it; scores far apart, all alike, and none at all"""
+    g, seqs, heads, new, length = rng(dim), 52, 4, 70, 100
+    host, values = filled_cache(q8, g, seqs, heads, 110, dim)
+    slots, starts, lens = list(range(seqs)), [new * b for b in range(seqs + 1)], [length] * seqs
+    poison_behind(host, slots, lens, True)
+    q = torch.randn(seqs * new, 2 * heads, dim, generator=g)
+    q[2 * new] *= 60
+    q[2 * new + 1] = 0
+    q = q.to(dtype)
+    cache = q8.KV8Cache(*(t.cuda() for t in host))
+    batch = make_batch(q8, slots, starts, lens)
+    for scale in (dim ** -0.5, 0.0):
+        check_attention(q8.kv_attention(q.cuda(), cache, batch, scale=scale), q, values, slots, starts, lens, True, scale, dtype)
+    host[1][0, 1, 90] = math.nan                                              # a key of head 1 of sequence 0
+    bad = q.clone()
+    bad[new + 7, 5, dim - 1] = math.inf                                       # a query of sequence 1
+    cache = q8.KV8Cache(*(t.cuda() for t in host))
+    clean = q8.kv_attention(q.cuda(), q8.KV8Cache(*(t.cuda() for t in [host[0], host[1].nan_to_num(0.01), host[2], host[3]])), batch).cpu()
+    got = q8.kv_attention(bad.cuda(), cache, batch).cpu()
+    want = torch.zeros(seqs * new, 2 * heads, dtype=torch.bool)
+    want[90 - (length - new):new, 2:4] = True
+    want[new + 7, 5] = True
+    assert torch.equal(torch.isnan(got).all(-1), want) and torch.equal(torch.isnan(got).any(-1), want)
+    assert torch.equal(got[~want], clean[~want])
 
 
 # ---- together ---------------------------------------------------------------------------------------------------------------------------
