@@ -483,7 +483,7 @@ int wj_comm_destroy(wj_comm* comm);
  * The operators of a decoder layer whose products run on 8-bit integers and whose key / value cache holds 8-bit codes: the
  * precision CTranslate2 offers the reference as compute_type="int8" (whisperjav/modules/faster_whisper_pro_asr.py:247-253 passes
  * compute_type on; weights in int8, activations quantised per row as they are produced), plus the cache.
- * A ROW of values x is held as int8 codes in [-127, 127] and one float32 scale: scale = max |x| / 127, code = x / scale rounded to
+ * A ROW of values x is held as int8 codes in [-127, 127] and one float32 scale: scale = max |x| / 127, code = 127 x / max |x| to the
  * nearest, ties to even; x reads back as code * scale, off by at most scale / 2.  A row of zeros has scale 0.  A row that holds a NaN or
  * an infinity has scale NaN and codes 0, so that it reads back as NaN and stays a single row's matter.
  * Every call is asynchronous on `stream` and may be captured into a graph (no allocation, no copy, no memset inside); `stream` =

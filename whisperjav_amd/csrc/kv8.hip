@@ -31,7 +31,7 @@ __device__ __forceinline__ Span span_of(const Kv8Args& a, int b) {
 
 // Writing: HD / 8 lanes hold one head's row of K and of V, 8 elements each, read and written with one wide access per lane and tensor; the
 // maximum goes over the lanes by exchanges.  Bound by memory: a 16-bit row of 128 moves 256 + 128 + 4 bytes; 20 k rows of 8 heads of K and V are
-// written in 31 us (4.1 TB/s) and read back in 23 (5.5).  A workgroup takes (row, head) pairs of one sequence in turn.
+// written in 26 us (4.9 TB/s) and read back in 21 (5.9).  A workgroup takes (row, head) pairs of one sequence in turn.
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void kv8_write_kernel(const Kv8Args a, const T* __restrict__ k, int64_t ldk, const T* __restrict__ v,
                                                         int64_t ldv) {

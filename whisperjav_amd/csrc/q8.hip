@@ -12,7 +12,7 @@ namespace {
 // Rows.  WPR waves hold one row in registers, 8 consecutive columns per lane and step (at most 4 steps): one read of the inputs, one
 // write of the outputs, the sum of squares and the maximum over lanes by shuffles (and over waves through LDS).  Bound by memory: the
 // norm of 16384 x 2048 float32 + float16 moves 11 bytes per element (369 MB with the weight) in 73 us, 5.0 TB/s, back to back in cold caches;
-// one row takes 4.3 us, which is the launch and two round trips.  Everything a row needs is requested before its first value is used.  Rows of any stride and base are read with wide loads (gfx950
+// one row takes 4.2 us, which is the launch and two round trips.  Everything a row needs is requested before its first value is used.  Rows of any stride and base are read with wide loads (gfx950
 // serves unaligned ones).  One wave per row when there are rows to fill the chip with (no barrier between the passes); else 4, which
 // shortens the chain of loads of a call that is bound by latency (see pick_rows).
 // --------------------------------------------------------------------------------------------
@@ -200,8 +200,8 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : WPR * 64) void q8_rows_kernel(cons
   if (tid == 0) a.scale[r] = q.scale;
 }
 
-// Read-back: a workgroup takes whole rows' groups of 8 columns in turn, one wide load and store each.  16383 x 2040 to bfloat16 (100 MB): 15.4 us, 6.5
-// TB/s, the codes partly from the caches they were just written to.
+// Read-back: a workgroup takes whole rows' groups of 8 columns in turn, one wide load and store each.  16383 x 2040 to bfloat16 (100 MB): 15 to 20 us, 5 TB/s
+// and more where the codes are still in the caches that they were written to.
 template <typename T>
 __global__ __launch_bounds__(256) void q8_dequantize_kernel(const int8_t* __restrict__ codes, int64_t ldc, const float* __restrict__ scale,
                                                             T* __restrict__ out, int64_t ldo, int64_t rows, int cols) {

@@ -1,7 +1,7 @@
 """8-bit operators of a decoder step on torch tensors (``wj_q8_*`` / ``wj_kv8_*``, ``include/wjhip.h``).
 
-A row of values is held as int8 codes in [-127, 127] and one float32 scale (max |x| / 127): ``rmsnorm`` and ``quantize`` produce such
-rows, ``gemm`` multiplies them with weights held the same way (a scale per token and per channel), ``KV8Cache`` holds keys and values
+A row of values is held as int8 codes in [-127, 127], 127 x / max |x| to the nearest, and one float32 scale, max |x| / 127: ``rmsnorm`` and ``quantize``
+produce such rows, ``gemm`` multiplies them with weights held the same way (a scale per token and per channel), ``KV8Cache`` holds keys and values
 like that, ``kv_write`` / ``kv_read`` / ``kv_attention`` fill, read back and attend to it.
 
 Every function launches on torch's current stream of the tensors' device and returns at once; outputs come from torch's allocator.  The
@@ -15,7 +15,7 @@ A decoder layer::
     ...                                                                         # head norms, rotary embedding
     q8.kv_write(cache, k, v, batch)
     o = q8.kv_attention(q, cache, batch)
-    attn_out = q8.gemm(*q8.quantize(o), w_o, w_o_scale)
+    attn_out = q8.gemm(*q8.quantize(o.flatten(1)), w_o, w_o_scale)
     codes, scale = q8.rmsnorm(x, ln2, eps, delta=attn_out)
     gate_up = q8.gemm(codes, scale, w_gate_up, w_gate_up_scale)
     mlp_out = q8.gemm(*q8.quantize(gate_up, swiglu_block=16), w_down, w_down_scale)
