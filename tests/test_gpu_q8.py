@@ -618,8 +618,13 @@ def test_refusals_on_the_device(q8):
     grad = torch.zeros(4, 64, device="cuda", requires_grad=True)
     with pytest.raises(ValueError, match="gradient"):
         q8.quantize(grad)
+    with pytest.raises(ValueError, match="gradient"):
+        q8.rmsnorm(x, w.clone().requires_grad_())
+    with pytest.raises(ValueError, match="gradient"):
+        q8.gemm(codes, scale, codes, scale, bias=torch.zeros(4, device="cuda", requires_grad=True))
     with torch.no_grad():
         q8.quantize(grad)
+        q8.rmsnorm(x, w.clone().requires_grad_())
     with pytest.raises(WjError):
         q8.quantize(torch.zeros(1, 32769).cuda())
     with pytest.raises(ValueError):

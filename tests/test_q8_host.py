@@ -1,4 +1,5 @@
 """The 8-bit operators without a GPU: what they refuse before anything is launched, and the plain forms the GPU tests compare with."""
+import copy
 import ctypes as C
 import math
 
@@ -46,6 +47,17 @@ def test_null_arguments_are_refused_at_the_c_entries(hip):
 
 def test_struct_layouts():
     assert C.sizeof(q8.Kv8C) == 48 and C.sizeof(q8.Kv8BatchC) == 40
+
+
+def test_copies_describe_their_own_tensors():
+    """a cache and a batch that were used hold addresses: a copy must not take them over"""
+    cache = q8.KV8Cache.empty(1, 1, 4, 64, torch.device("cpu"))
+    batch = q8.Batch(*(torch.zeros(n, dtype=torch.int32) for n in (1, 2, 1)), 1, 1)
+    cache.__dict__["_c"], batch.__dict__["_c"] = q8.Kv8C(), (1, 0, q8.Kv8BatchC())
+    for used in (cache, batch):
+        for other in (copy.deepcopy(used), copy.copy(used), used._replace()):
+            assert type(other) is type(used) and "_c" not in other.__dict__ and len(other) == len(used)
+    assert copy.deepcopy(cache).k.data_ptr() != cache.k.data_ptr()
 
 
 def test_plain_quantiser():

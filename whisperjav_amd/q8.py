@@ -92,6 +92,8 @@ def _codes(t: torch.Tensor, scale: torch.Tensor, what: str, index: Optional[int]
 def _vector(t: torch.Tensor, what: str, n: int, index: int) -> None:
     if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or t.get_device() != index:
         raise ValueError(f"{what}: contiguous float32 [{n}] on cuda:{index} expected, got {t.dtype} {list(t.shape)} on {t.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: requires a gradient; these operators have none (torch.no_grad() to go on)")
 
 
 def _output(t: torch.Tensor, what: str) -> None:
@@ -110,7 +112,8 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, delta: 
             residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scale)`` of the rows of ``(x + delta) / rms(x + delta) * weight``.
 
-    ``residual`` receives ``x + delta`` in x's type; left out, the sum is written back into ``x`` (when there is a ``delta``)."""
+    ``residual`` receives ``x + delta`` in x's type; left out, the sum is written back into ``x`` (when there is a ``delta``).  The squares
+    are summed in float32, as in the plain form: their sum must stay below 3e38."""
     xt = _float_rows(x, "x")
     rows, cols = x.shape
     index = x.get_device()
@@ -220,6 +223,9 @@ class KV8Cache(_CacheTensors):
             return torch.zeros((slots, heads, ctx), dtype=torch.float32, device=device)
         return cls(codes(), scale(), codes(), scale())
 
+    def __reduce__(self):                        # a copy describes its own tensors
+        return type(self), tuple(self)
+
 
 class _BatchArrays(NamedTuple):
     slots: torch.Tensor
@@ -234,6 +240,9 @@ class Batch(_BatchArrays):
     ``lens[b]`` positions in slot ``slots[b]`` of the cache once they are written, the rows being the last ones.  A slot of -1 is padding.
     ``max_new`` / ``max_len``: the most new rows / positions of any sequence; they size the launch (results do not depend on them).  The
     arrays may change between replays of a captured graph.  Slots are distinct where the batch is written."""
+
+    def __reduce__(self):
+        return type(self), tuple(self)
 
 
 def _cache(cache: KV8Cache) -> Kv8C:
