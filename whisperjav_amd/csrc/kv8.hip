@@ -101,10 +101,10 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, T* __res
 // Weights: with x = scale * log2(e) * ks * (q . k), the numerator of a position is 2^x vs, and 16 bits must hold it whatever the
 // scales are.  So the running reference of a row is M = max(x + exponent of vs) - 11, numerators are 2^(x - M) vs (at most 2^15), the
 // denominator sums 2^(x - M) in float32.  M moves only when the largest numerator would pass 2^15.  The smallest step of a half, 2^-24, is then
-// 2^-34 of the row's largest numerator or less: what a weight can lose for being small.  A numerator goes into the product as one half
-// for bfloat16 rows (2^-12 of a weight, an eighth of what rounding the output costs) and as a high and a low half (22 bits) for float16
-// and float32 rows: with one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 (512 sequences; 124 us either way, the
-// matrix pipe has room).
+// 2^-34 of the row's largest numerator or less: what a weight can lose for being small.  A numerator goes into the product as a high and a low
+// half (21 bits or more): the results are those of the float32 form.  With one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 and
+// a bfloat16 row 1.671e-3 instead of 1.658e-3 (8 % of its values are not the nearest ones, against 0.06 %); the second product costs nothing where
+// memory bounds the call (512 sequences 124 us) and 10 % of a bfloat16 prompt pass (32 prompts 142 -> 157 us).
 // --------------------------------------------------------------------------------------------
 struct AttnArgs {
   Kv8Args s;
@@ -120,6 +120,19 @@ struct AttnArgs {
 
 constexpr float kRoom = 11.f, kSlack = 15.f;
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+
+// Eight numerators as high and low halves.  The high ones are cut off instead of rounded, two at an instruction: the low ones hold what is left.
+__device__ __forceinline__ void split_halves(const float (&w)[8], f16x8_t (&out)[2]) {
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(w[2 * j], w[2 * j + 1]);
+    hi[j] = __builtin_bit_cast(uint32_t, h);
+    lo[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(w[2 * j] - (float)h[0], w[2 * j + 1] - (float)h[1]));
+  }
+  out[0] = __builtin_bit_cast(f16x8_t, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+  out[1] = __builtin_bit_cast(f16x8_t, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+}
 
 __device__ __forceinline__ uint32_t h2_less(uint32_t w) {      // two halves, 1152 taken off each
   const h2_t c = {(_Float16)1152.f, (_Float16)1152.f};
@@ -252,7 +265,6 @@ template <int N> struct Part {
 template <typename T, int HD, int RT, int NV>      // NV waves
 __global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv8_attn_rows_kernel(const AttnArgs a) {
   constexpr int NP = sizeof(T) == 4 ? 2 : 1;                              // halves of a query
-  constexpr int NW = std::is_same<T, bf16_t>::value ? 1 : 2;              // halves of a weight
   constexpr int NE = HD / 16;                  // 16-dim tiles of the output; a lane's output dims are NE consecutive ones, four times
   constexpr int KW = HD / 64;                  // 16-byte pieces of a key per lane
   constexpr int LDO = HD + 4;
@@ -344,7 +356,7 @@ __global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv
             }
         }
       }
-      f16x8_t pf[RT][NW];
+      f16x8_t pf[RT][2];
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         float x[8], top = -INFINITY;
@@ -365,16 +377,15 @@ __global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv
             for (int r = 0; r < 4; ++r) o[t][e][r] *= f;
         }
         const float m = M[t] == -INFINITY ? 0.f : M[t];
+        float w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool in = !MASKED || kt + 8 * lg + j < limit[t];
           const float p = in ? __builtin_amdgcn_exp2f(fmaf(x[j], unit[t], -m)) : 0.f;
           l[t] += p;
-          const float w = in ? p * vs[j] : 0.f;
-          const f16_t hi = f2h(w);
-          pf[t][0][j] = hi;
-          if constexpr (NW == 2) pf[t][1][j] = f2h(w - h2f(hi));
+          w[j] = in ? p * vs[j] : 0.f;
         }
+        split_halves(w, pf[t]);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -389,7 +400,7 @@ __global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int p = 0; p < NW; ++p) o[t][E] = mfma16(vf, pf[t][p], o[t][E]);
+          for (int p = 0; p < 2; ++p) o[t][E] = mfma16(vf, pf[t][p], o[t][E]);
       };
       value_tile(std::integral_constant<int, 0>{}); value_tile(std::integral_constant<int, 1>{});
       value_tile(std::integral_constant<int, 2>{}); value_tile(std::integral_constant<int, 3>{});
@@ -452,7 +463,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void* p, int bytes) 
 // workgroup); 4 of 4000 positions, 32 heads on 8, 690 us, 760 TFLOP/s of what the causal mask leaves.
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a, int blocks) {
-  constexpr int NP = 1, NW = std::is_same<T, bf16_t>::value ? 1 : 2;
+  constexpr int NP = 1;
   constexpr int NE = HD / 16, KS = HD / 32;
   constexpr int KB = 64 * HD * 2, VB = 64 * HD * 2, BUF = KB + VB + 3 * 256;       // K [64][HD], V^T [HD][64], then ks, vs, exponents [64]
   constexpr int KL = HD / 64;                                                      // 16-byte pieces of K per thread
@@ -579,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
             for (int p = 0; p < NP; ++p) st[t][kb] = mfma16(kf, qf[t][p][c], st[t][kb]);
         }
       }
-      f16x8_t pf[2][NW];
+      f16x8_t pf[2][2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         float x[8], top = -INFINITY;
@@ -600,16 +611,15 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
             for (int r = 0; r < 4; ++r) o[t][e][r] *= f;
         }
         const float m = M[t] == -INFINITY ? 0.f : M[t];
+        float w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool in = !MASKED || key0 + j < limit[t];
           const float p = in ? __builtin_amdgcn_exp2f(fmaf(x[j], unit[t], -m)) : 0.f;
           l[t] += p;
-          const float w = in ? p * vs[j] : 0.f;
-          const f16_t hi = f2h(w);
-          pf[t][0][j] = hi;
-          if constexpr (NW == 2) pf[t][1][j] = f2h(w - h2f(hi));
+          w[j] = in ? p * vs[j] : 0.f;
         }
+        split_halves(w, pf[t]);
       }
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
@@ -617,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int p = 0; p < NW; ++p) o[t][e] = mfma16(vf, pf[t][p], o[t][e]);
+          for (int p = 0; p < 2; ++p) o[t][e] = mfma16(vf, pf[t][p], o[t][e]);
       }
     };
 
