@@ -100,10 +100,12 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, T* __res
 //
 // Weights: with x = scale * log2(e) * ks * (q . k), the numerator of a position is 2^x vs, and 16 bits must hold it whatever the
 // scales are.  So the running reference of a row is M = max(x + exponent of vs) - 11, numerators are 2^(x - M) vs (at most 2^15), the
-// denominator sums 2^(x - M) in float32.  M moves only when the largest numerator would pass 2^15.  The smallest step of a half, 2^-24, is then
-// 2^-34 of the row's largest numerator or less: what a weight can lose for being small.  A numerator goes into the product as a high and a low
-// half (21 bits or more): the results are those of the float32 form.  With one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 and
-// a bfloat16 row 1.671e-3 instead of 1.658e-3 (8 % of its values are not the nearest ones, against 0.06 %); the second product costs nothing where
+// denominator sums 2^(x - M) in float32.  A scale has an exponent of up to 128, which puts the denominator's terms down at 2^-117, where the exponential
+// gives nothing below 2^-126: M and with it the exponentials are carried 20 binades higher, the scales and the denominator's terms taken 20 lower.
+// Exponents below -90 count as -90, so that a term is at most 2^105: scales below 2^-105 lose bits of their numerators.
+// M moves only when the largest numerator would pass 2^15.  The smallest step of a half, 2^-24, is then 2^-34 of the row's largest numerator or
+// less: what a weight can lose for being small.  A numerator goes into the product as a high and a low half (21 bits or more): the results are
+// those of the float32 form.  With one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 and a bfloat16 row 1.671e-3 instead of 1.658e-3 (8 % of its values are not the nearest ones, against 0.06 %); the second product costs nothing where
 // memory bounds the call (512 sequences 124 us) and 10 % of a bfloat16 prompt pass (32 prompts 142 -> 157 us).
 // --------------------------------------------------------------------------------------------
 struct AttnArgs {
@@ -118,7 +120,7 @@ struct AttnArgs {
   float2* ml;                // ... and (M, denominator)
 };
 
-constexpr float kRoom = 11.f, kSlack = 15.f;
+constexpr float kRoom = 31.f, kSlack = 35.f, kDown = 0x1p-20f;
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 
 // Eight numerators as high and low halves.  The high ones are cut off instead of rounded, two at an instruction: the low ones hold what is left.
@@ -167,7 +169,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 }
 
 __device__ __forceinline__ float scale_exponent(float vs) {      // of a value scale, bounded so that 2^(x - M) and its sums stay in range
-  return vs == 0.f ? -90.f : fminf(fmaxf((float)__builtin_amdgcn_frexp_expf(vs), -90.f), 110.f);
+  return vs == 0.f ? -90.f : fmaxf((float)__builtin_amdgcn_frexp_expf(vs), -90.f);
 }
 
 __device__ __forceinline__ int over_per(const AttnArgs& a, int r) { return a.per == 1 ? r : (int)__umulhi((uint32_t)r, a.per_inv); }
@@ -242,14 +244,21 @@ template <typename T, int N> __device__ __forceinline__ void st_out(T* p, const 
   __builtin_memcpy(p, t, sizeof(t));
 }
 
+// A denominator brought to a reference that is -by higher, in two steps: beyond 2^-126 the factor would be zero.  The numerators add nothing to
+// the result then, but the denominator may hold the weights of positions whose values are that much smaller.
+__device__ __forceinline__ float lower_sum(float sum, float by) {
+  const float f = __builtin_amdgcn_exp2f(0.5f * by);
+  return sum * f * f;
+}
+
 // Parts of one row over different positions, each with its reference and denominator: brought to the largest reference and added.  A part
 // that saw nothing (reference -inf, zeros) adds nothing; one that holds a NaN makes one of the sum.
 template <int N> struct Part {
   float top = -INFINITY, sum = 0.f, o[N] = {};
   __device__ __forceinline__ void see(float2 ml) { top = fmaxf(top, ml.x); }
   __device__ __forceinline__ void add(float2 ml, const float* part) {
-    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
-    sum = fmaf(ml.y, f, sum);
+    const float by = ml.x - (top == -INFINITY ? 0.f : top), f = __builtin_amdgcn_exp2f(by);
+    sum += lower_sum(ml.y, by);
 #pragma unroll
     for (int e = 0; e < N; ++e) o[e] = fmaf(part[e], f, o[e]);
   }
@@ -338,7 +347,7 @@ __global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv
       }
       float ex[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ex[j] = scale_exponent(vs[j]);
+      for (int j = 0; j < 8; ++j) { ex[j] = scale_exponent(vs[j]); vs[j] *= kDown; }
       f32x4_t st[RT][2];
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
@@ -368,9 +377,9 @@ __global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv
         }
         top = quad_max(top);
         if (top > M[t] + kSlack) {
-          const float f = __builtin_amdgcn_exp2f(M[t] - (top - kRoom));      // the first time: 0 on zeros
+          const float by = M[t] - (top - kRoom), f = __builtin_amdgcn_exp2f(by);      // the first time: 0 on zeros
           M[t] = top - kRoom;
-          l[t] *= f;
+          l[t] = lower_sum(l[t], by);
 #pragma unroll
           for (int e = 0; e < NE; ++e)
 #pragma unroll
@@ -382,7 +391,7 @@ __global__ __launch_bounds__(NV * 64, sizeof(T) == 4 && RT == 2 ? 1 : 2) void kv
         for (int j = 0; j < 8; ++j) {
           const bool in = !MASKED || kt + 8 * lg + j < limit[t];
           const float p = in ? __builtin_amdgcn_exp2f(fmaf(x[j], unit[t], -m)) : 0.f;
-          l[t] += p;
+          l[t] = fmaf(p, kDown, l[t]);
           w[j] = in ? p * vs[j] : 0.f;
         }
         split_halves(w, pf[t]);
@@ -465,7 +474,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a, int blocks) {
   constexpr int NP = 1;
   constexpr int NE = HD / 16, KS = HD / 32;
-  constexpr int KB = 64 * HD * 2, VB = 64 * HD * 2, BUF = KB + VB + 3 * 256;       // K [64][HD], V^T [HD][64], then ks, vs, exponents [64]
+  constexpr int KB = 64 * HD * 2, VB = 64 * HD * 2, BUF = KB + VB + 3 * 256;       // K [64][HD], V^T [HD][64], then ks, 2^-20 vs, exponents of vs [64]
   constexpr int KL = HD / 64;                                                      // 16-byte pieces of K per thread
   extern __shared__ __attribute__((aligned(16))) char lds_t[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, lg = lane >> 4;
@@ -534,8 +543,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
         *reinterpret_cast<uint4*>(v2 + 384) = make_uint4(codes_pair<3>(w[0], w[1]), codes_pair<3>(w[2], w[3]), codes_pair<3>(w[4], w[5]), codes_pair<3>(w[6], w[7]));
       }
       float* sc = reinterpret_cast<float*>(b + KB + VB);
-      if (tid < 128) sc[tid] = __uint_as_float(rs);
-      if (tid >= 64 && tid < 128) sc[64 + tid] = scale_exponent(__uint_as_float(rs));
+      if (tid < 64) sc[tid] = __uint_as_float(rs);
+      else if (tid < 128) { sc[tid] = __uint_as_float(rs) * kDown; sc[64 + tid] = scale_exponent(__uint_as_float(rs)); }
     };
 
     if (kend > 0) fetch(0);                // in flight while the queries are read
@@ -602,9 +611,9 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
         }
         top = quad_max(top);
         if (top > M[t] + kSlack) {
-          const float f = __builtin_amdgcn_exp2f(M[t] - (top - kRoom));
+          const float by = M[t] - (top - kRoom), f = __builtin_amdgcn_exp2f(by);
           M[t] = top - kRoom;
-          l[t] *= f;
+          l[t] = lower_sum(l[t], by);
 #pragma unroll
           for (int e = 0; e < NE; ++e)
 #pragma unroll
@@ -616,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a,
         for (int j = 0; j < 8; ++j) {
           const bool in = !MASKED || key0 + j < limit[t];
           const float p = in ? __builtin_amdgcn_exp2f(fmaf(x[j], unit[t], -m)) : 0.f;
-          l[t] += p;
+          l[t] = fmaf(p, kDown, l[t]);
           w[j] = in ? p * vs[j] : 0.f;
         }
         split_halves(w, pf[t]);
