@@ -2,6 +2,7 @@
 #include <type_traits>
 
 #include "q8.hpp"
+#include "q8_plan.hpp"
 
 using namespace wj;
 
@@ -12,21 +13,10 @@ struct Kv8Args {
   wj_kv8_batch b;
 };
 
-// What a sequence of the call owns.  first .. first + n - 1: its rows of the row arrays; pos0: position of the first of them
-struct Span { int slot, first, n, len, pos0; };
 __device__ __forceinline__ Span span_of(const Kv8Args& a, int b) {
   // the same for every lane: kept in scalar registers
   auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  Span s;
-  s.slot = uni(a.b.slots_dev[b]);
-  s.first = uni(a.b.starts_dev[b]);
-  const int last = min(uni(a.b.starts_dev[b + 1]), a.b.rows);
-  if (s.first < 0) s.first = a.b.rows;                 // not a span of the arrays: no rows
-  s.n = max(0, last - s.first);
-  s.len = uni(a.b.lens_dev[b]);
-  s.pos0 = s.len - s.n;
-  if (s.slot < 0 || s.slot >= a.c.slots) s.slot = -1;
-  return s;
+  return span_from(uni(a.b.slots_dev[b]), uni(a.b.starts_dev[b]), uni(a.b.starts_dev[b + 1]), uni(a.b.lens_dev[b]), a.c.slots, a.b.rows);
 }
 
 // Writing: HD / 8 lanes hold one head's row of K and of V, 8 elements each, read and written with one wide access per lane and tensor; the
