@@ -37,3 +37,57 @@ def test_arrays_that_are_no_spans(q8, starts, lens):
         assert torch.equal(out[:3], want[:3]) and bool((out[3:rows] == 0).all()) and bool((out[rows:] == 9).all())
     back = q8.kv_read(cache, batch, 6, torch.float32)
     assert torch.equal(back[0][:3], q8.kv_read(good, one, 6, torch.float32)[0][:3]) and bool((back[0][3:rows] == 0).all())
+
+
+def layer_inputs(q8):
+    g = torch.Generator().manual_seed(2)
+    x, d = torch.randn(4, 64, generator=g).cuda(), torch.randn(4, 64, generator=g).cuda()
+    codes, scale = q8.quantize(x)
+    cache = q8.KV8Cache.empty(1, 1, 8, 64)
+    return x, d, codes, scale, cache, q8.Batch(ints([0]), ints([0, 4]), ints([4]), 4, 4), torch.ones(64).cuda()
+
+
+def writers(q8):
+    """name -> (the tensor that is written, the call)"""
+    x, d, codes, scale, cache, batch, w = layer_inputs(q8)
+    rows, res, out, att = x.view(4, 1, 64), torch.zeros_like(x), torch.zeros(4, 4).cuda(), torch.zeros(4, 1, 64).cuda()
+    return {
+        "rmsnorm in place": (x, lambda: q8.rmsnorm(x, w, delta=d)),
+        "rmsnorm residual": (res, lambda: q8.rmsnorm(x, w, residual=res)),
+        "gemm out": (out, lambda: q8.gemm(codes, scale, codes, scale, out=out)),
+        "attention out": (att, lambda: q8.kv_attention(rows, cache, batch, out=att)),
+        "cache k": (cache.k_scale, lambda: q8.kv_write(cache, rows, rows, batch)),
+        "cache v": (cache.v_scale, lambda: q8.kv_write(cache, rows, rows, batch)),
+    }
+
+
+@pytest.mark.parametrize("name", ["rmsnorm in place", "rmsnorm residual", "gemm out", "attention out", "cache k", "cache v"])
+def test_a_backward_that_saved_what_is_written_raises(q8, name):
+    written, call = writers(q8)[name]
+    p = torch.ones(written.shape, device="cuda", requires_grad=True)
+    loss = (written * p).sum()                               # saves `written` for p's gradient
+    call()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_what_is_only_read_keeps_its_version(q8):
+    x, d, codes, scale, cache, batch, w = layer_inputs(q8)
+    read = [x, d, codes, scale, w, *cache, *batch[:3]]
+    before = [t._version for t in read]
+    q8.rmsnorm(x, w)
+    q8.rmsnorm(x, w, delta=d, residual=torch.empty_like(x))
+    q8.dequantize(*q8.quantize(x))
+    q8.gemm(codes, scale, codes, scale)
+    q8.kv_attention(x.view(4, 1, 64), cache, batch)
+    q8.kv_read(cache, batch, 4)
+    assert [t._version for t in read] == before
+
+
+def test_tensors_of_inference_mode_are_served(q8):
+    with torch.inference_mode():
+        calls = writers(q8)
+        for _, call in calls.values():
+            call()
+    for _, call in calls.values():
+        call()

@@ -5,7 +5,8 @@ produce such rows, ``gemm`` multiplies them with weights held the same way (a sc
 like that, ``kv_write`` / ``kv_read`` / ``kv_attention`` fill, read back and attend to it.
 
 Every function launches on torch's current stream of the tensors' device and returns at once; outputs come from torch's allocator.  The
-calls may be captured into a ``torch.cuda.graph``.  They serve inference and refuse tensors that want a gradient.  Arguments are checked
+calls may be captured into a ``torch.cuda.graph``.  They serve inference and refuse tensors that want a gradient.  What they
+write in place (``x`` or ``residual``, ``out``, the cache) is marked as modified, so that a ``backward`` which saved it raises.  Arguments are checked
 on the host (``ValueError``); the library's own refusals raise ``hipbind.WjError``.  There is no CPU path.
 
 A decoder layer::
@@ -26,6 +27,7 @@ import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version as _modified
 
 from . import hipbind
 from .hipbind import WJ_BF16, WJ_F16, WJ_F32
@@ -59,6 +61,11 @@ def _fail(name: str, rc: int) -> None:
     hipbind.check(rc, name)
 
 
+def _no_gradient(t: torch.Tensor, what: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: requires a gradient; these operators have none (torch.no_grad() to go on)")
+
+
 def _float_rows(t: torch.Tensor, what: str, index: Optional[int] = None, rows: int = -1, cols: int = -1) -> int:
     """Check a ``[rows, cols]`` float tensor whose rows are contiguous (on GPU ``index``); its type code."""
     code = _TYPE.get(t.dtype)
@@ -71,8 +78,7 @@ def _float_rows(t: torch.Tensor, what: str, index: Optional[int] = None, rows: i
         raise ValueError(f"{what}: on {t.device}, expected {'a GPU' if index is None else f'cuda:{index}'}")
     if t.stride(1) != 1 and shape[1] > 1:
         raise ValueError(f"{what}: the elements of a row must be contiguous (stride {t.stride(1)})")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: requires a gradient; these operators have none (torch.no_grad() to go on)")
+    _no_gradient(t, what)
     return code
 
 
@@ -92,8 +98,7 @@ def _codes(t: torch.Tensor, scale: torch.Tensor, what: str, index: Optional[int]
 def _vector(t: torch.Tensor, what: str, n: int, index: int) -> None:
     if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1) or t.get_device() != index:
         raise ValueError(f"{what}: contiguous float32 [{n}] on cuda:{index} expected, got {t.dtype} {list(t.shape)} on {t.device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: requires a gradient; these operators have none (torch.no_grad() to go on)")
+    _no_gradient(t, what)
 
 
 def _output(t: torch.Tensor, what: str) -> None:
@@ -137,6 +142,8 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *, delta: 
                            scale.data_ptr(), rows, cols, stream)
     if rc:
         _fail("wj_q8_rmsnorm", rc)
+    if residual is not None:
+        _modified(residual)
     return codes, scale
 
 
@@ -184,6 +191,7 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
         raise ValueError(f"a has {k} columns, w has {w.shape[1]}")
     if bias is not None:
         _vector(bias, "bias", n, index)
+    given = out
     if out is None:
         dt = _TYPE.get(dtype)
         if dt is None:
@@ -200,6 +208,8 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
                         work.data_ptr() if need else None, need, stream)
     if rc:
         _fail("wj_q8_gemm", rc)
+    if given is not None:
+        _modified(given)
     return out
 
 
@@ -246,10 +256,10 @@ class Batch(_BatchArrays):
 
 
 def _cache(cache: KV8Cache) -> Kv8C:
+    k, ks, v, vs = cache
     c = cache.__dict__.get("_c")                 # checked and laid out at the object's first use
     if c is not None:
         return c
-    k, ks, v, vs = cache
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
         raise ValueError(f"cache: codes [slots, heads, ctx, dim] and scales [slots, heads, ctx] expected, got {list(k.shape)}, {list(ks.shape)}, "
@@ -288,8 +298,7 @@ def _head_rows(t: torch.Tensor, what: str, cache: Kv8C, index: int, heads: Optio
         raise ValueError(f"{what}: float32, float16 or bfloat16 expected, got {t.dtype}")
     if t.get_device() != index:
         raise ValueError(f"{what}: on {t.device}, expected cuda:{index}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: requires a gradient; these operators have none (torch.no_grad() to go on)")
+    _no_gradient(t, what)
     stride = t.stride()
     if stride[2] != 1 or (shape[1] > 1 and stride[1] != cache.dim):
         raise ValueError(f"{what}: the heads of a row must lie one after the other, their elements too (strides {stride})")
@@ -307,6 +316,7 @@ def kv_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, batch: Batch) ->
     rc = lib.wj_kv8_write(ctx, C.byref(c), C.byref(b), dt, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), stream)
     if rc:
         _fail("wj_kv8_write", rc)
+    _modified(cache)
 
 
 def kv_read(cache: KV8Cache, batch: Batch, rows: int, dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -335,6 +345,7 @@ def kv_attention(q: torch.Tensor, cache: KV8Cache, batch: Batch, *, causal: bool
     c, index = _cache(cache), cache.k.get_device()
     dt = _head_rows(q, "q", c, index)
     rows, heads, dim = q.shape
+    given = out
     if out is None:
         out = torch.empty(rows, heads, dim, dtype=q.dtype, device=q.device)
     elif _head_rows(out, "out", c, index, heads) != dt or out.shape[0] != rows or (rows > 1 and out.stride(0) < heads * dim):
@@ -348,4 +359,6 @@ def kv_attention(q: torch.Tensor, cache: KV8Cache, batch: Batch, *, causal: bool
                               1 if causal else 0, work.data_ptr() if need else None, need, stream)
     if rc:
         _fail("wj_kv8_attention", rc)
+    if given is not None:
+        _modified(given)
     return out
