@@ -91,3 +91,32 @@ def test_tensors_of_inference_mode_are_served(q8):
             call()
     for _, call in calls.values():
         call()
+
+
+def test_tangents_and_gradients_are_refused(q8):
+    import torch.autograd.forward_ad as forward
+    x, d, codes, scale, cache, batch, w = layer_inputs(q8)
+    rows = x.view(4, 1, 64)
+
+    def calls(wrap):
+        return [lambda: q8.quantize(wrap(x)), lambda: q8.rmsnorm(wrap(x), w), lambda: q8.rmsnorm(x, wrap(w)), lambda: q8.rmsnorm(x, w, delta=wrap(d)),
+                lambda: q8.rmsnorm(x, w, residual=wrap(d)), lambda: q8.dequantize(codes, wrap(scale)), lambda: q8.gemm(codes, wrap(scale), codes, scale),
+                lambda: q8.gemm(codes, scale, codes, scale, bias=wrap(scale)), lambda: q8.kv_write(cache, wrap(rows), rows, batch),
+                lambda: q8.kv_write(cache, rows, wrap(rows), batch), lambda: q8.kv_attention(wrap(rows), cache, batch),
+                lambda: q8.kv_attention(rows, cache._replace(v_scale=wrap(cache.v_scale)), batch),
+                lambda: q8.kv_read(cache._replace(k_scale=wrap(cache.k_scale)), batch, 4)]
+    with forward.dual_level():
+        for call in calls(lambda t: forward.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        q8.rmsnorm(x, w)                                     # tensors without one go on
+    for call in calls(lambda t: t.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    used = cache._replace(v_scale=cache.v_scale.clone())
+    q8.kv_attention(rows, used, batch)
+    used.v_scale.requires_grad_()                            # ... after its first use too
+    with pytest.raises(ValueError, match="gradient"):
+        q8.kv_attention(rows, used, batch)

@@ -5,7 +5,7 @@ produce such rows, ``gemm`` multiplies them with weights held the same way (a sc
 like that, ``kv_write`` / ``kv_read`` / ``kv_attention`` fill, read back and attend to it.
 
 Every function launches on torch's current stream of the tensors' device and returns at once; outputs come from torch's allocator.  The
-calls may be captured into a ``torch.cuda.graph``.  They serve inference and refuse tensors that want a gradient.  What they
+calls may be captured into a ``torch.cuda.graph``.  They serve inference and refuse tensors that want a gradient or carry a tangent.  What they
 write in place (``x`` or ``residual``, ``out``, the cache) is marked as modified, so that a ``backward`` which saved it raises.  Arguments are checked
 on the host (``ValueError``); the library's own refusals raise ``hipbind.WjError``.  There is no CPU path.
 
@@ -27,6 +27,7 @@ import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward
 from torch.autograd.graph import increment_version as _modified
 
 from . import hipbind
@@ -64,6 +65,8 @@ def _fail(name: str, rc: int) -> None:
 def _no_gradient(t: torch.Tensor, what: str) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: requires a gradient; these operators have none (torch.no_grad() to go on)")
+    if _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what}: carries a tangent; these operators have none")
 
 
 def _float_rows(t: torch.Tensor, what: str, index: Optional[int] = None, rows: int = -1, cols: int = -1) -> int:
@@ -257,6 +260,8 @@ class Batch(_BatchArrays):
 
 def _cache(cache: KV8Cache) -> Kv8C:
     k, ks, v, vs = cache
+    _no_gradient(ks, "cache scale")
+    _no_gradient(vs, "cache scale")
     c = cache.__dict__.get("_c")                 # checked and laid out at the object's first use
     if c is not None:
         return c
