@@ -120,3 +120,27 @@ def test_tangents_and_gradients_are_refused(q8):
     used.v_scale.requires_grad_()                            # ... after its first use too
     with pytest.raises(ValueError, match="gradient"):
         q8.kv_attention(rows, used, batch)
+
+
+def test_arrays_and_caches_whose_memory_moved(q8):
+    """a used batch or cache whose tensors were given other memory: the new memory counts, and is checked (what was there before may be freed)"""
+    x, d, codes, scale, cache, batch, w = layer_inputs(q8)
+    rows = x.view(4, 1, 64)
+    q8.kv_write(cache, rows, rows, batch)
+    q8.kv_attention(rows, cache, batch)
+    batch.lens.data = ints([2])                              # two of the four rows lie before position 0 now
+    want = q8.kv_attention(rows, cache, q8.Batch(ints([0]), ints([0, 4]), ints([2]), 4, 4))
+    assert torch.equal(q8.kv_attention(rows, cache, batch), want)
+    other = q8.KV8Cache.empty(1, 1, 8, 64)
+    q8.kv_write(other, d.view(4, 1, 64), rows, batch)
+    cache.k.data, cache.k_scale.data, cache.v.data, cache.v_scale.data = (t.clone() for t in other)
+    assert torch.equal(q8.kv_attention(rows, cache, batch), q8.kv_attention(rows, other, batch))
+    q8.kv_write(cache, rows, rows, batch)                    # goes to the new memory, not to the other cache's
+    assert not torch.equal(cache.k, other.k)
+    batch.lens.data = ints([2, 3])
+    with pytest.raises(ValueError, match="lens"):
+        q8.kv_attention(rows, cache, batch)
+    batch.lens.data = ints([2])
+    cache.v_scale.data = torch.zeros(1, 1, 7).cuda()
+    with pytest.raises(ValueError, match="scales"):
+        q8.kv_attention(rows, cache, batch)

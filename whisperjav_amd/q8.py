@@ -225,7 +225,7 @@ class _CacheTensors(NamedTuple):
 
 class KV8Cache(_CacheTensors):
     """One layer's keys and values in 8 bits: codes int8 ``[slots, heads, ctx, dim]`` and scales float32 ``[slots, heads, ctx]``.
-    A program keeps it like a handle: the tensors are checked at its first use, and their memory has to stay where it is."""
+    A program keeps it like a handle: the tensors are checked at its first use, and again when one of them has other memory or another size."""
 
     @classmethod
     def empty(cls, slots: int, heads: int, ctx: int, dim: int, device: torch.device = torch.device("cuda", 0)) -> "KV8Cache":
@@ -262,9 +262,10 @@ def _cache(cache: KV8Cache) -> Kv8C:
     k, ks, v, vs = cache
     _no_gradient(ks, "cache scale")
     _no_gradient(vs, "cache scale")
-    c = cache.__dict__.get("_c")                 # checked and laid out at the object's first use
-    if c is not None:
-        return c
+    at = (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), k.numel(), ks.numel(), v.numel(), vs.numel())
+    known = cache.__dict__.get("_c")             # checked and laid out at the object's first use
+    if known is not None and known[0] == at:
+        return known[1]
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or ks.shape != shape[:3] or vs.shape != shape[:3]:
         raise ValueError(f"cache: codes [slots, heads, ctx, dim] and scales [slots, heads, ctx] expected, got {list(k.shape)}, {list(ks.shape)}, "
@@ -275,21 +276,23 @@ def _cache(cache: KV8Cache) -> Kv8C:
         raise ValueError("cache: the four tensors must be on one GPU")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache: contiguous tensors expected")
-    c = cache.__dict__["_c"] = Kv8C(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), *shape)
+    c = Kv8C(*at[:4], *shape)
+    cache.__dict__["_c"] = (at, c)
     return c
 
 
 def _batch(batch: Batch, rows: int, index: int) -> Kv8BatchC:
-    known = batch.__dict__.get("_c")
-    if known is not None and known[0] == rows and known[1] == index:
-        return known[2]
     slots, starts, lens, max_new, max_len = batch
+    at = (slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), rows, index, slots.numel(), starts.numel(), lens.numel())
+    known = batch.__dict__.get("_c")
+    if known is not None and known[0] == at:
+        return known[1]
     n = slots.shape[0] if slots.dim() == 1 else -1
     for t, what, want in ((slots, "slots", n), (starts, "starts", n + 1), (lens, "lens", n)):
         if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != want or t.get_device() != index or not t.is_contiguous():
             raise ValueError(f"batch.{what}: contiguous int32 [{want if want >= 0 else 'seqs'}] on cuda:{index} expected, got {t.dtype} {list(t.shape)} on {t.device}")
-    b = Kv8BatchC(slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), n, rows, max_new, max_len)
-    batch.__dict__["_c"] = (rows, index, b)
+    b = Kv8BatchC(*at[:3], n, rows, max_new, max_len)
+    batch.__dict__["_c"] = (at, b)
     return b
 
 
