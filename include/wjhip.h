@@ -512,7 +512,7 @@ int wj_q8_dequantize(wj_ctx* ctx, const int8_t* codes_dev, int64_t ldc, const fl
  * (int32; codes may be -128 too, hence k <= 131071); the epilogue is float32, rounded once.  lda, ldw >= k.  Rows of codes that start at
  * multiples of 16 bytes take the fast kernels (bytes between k and the next multiple of 16 are read and ignored, never written); any
  * other base or stride is served, slower.  workspace_dev: at least wj_q8_gemm_workspace() bytes (may be 0 and NULL), used by this call
- * alone until it is done on `stream`. */
+ * alone until it is done on `stream`.  At most 4194240 rows and 2^27 - 16 columns. */
 int64_t wj_q8_gemm_workspace(wj_ctx* ctx, int64_t m, int n, int k);
 int wj_q8_gemm(wj_ctx* ctx, const int8_t* a_dev, int64_t lda, const float* a_scale_dev, const int8_t* w_dev, int64_t ldw,
                const float* w_scale_dev, const float* bias_dev, int dtype, void* out_dev, int64_t ldo, int64_t m, int n, int k,

@@ -78,3 +78,27 @@ def test_plain_attention_against_a_sum_written_out():
             want = sum(wi * v[1, 0, j] for j, wi in enumerate(w)) / sum(w)
             assert torch.allclose(got[t, h], want, atol=1e-12)
     assert bool((got[2] == 0).all())
+
+
+def meta(*shape, dtype=torch.int8):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("call", [
+    lambda: q8.quantize(meta(1, 2 ** 32 + 8, dtype=torch.float16)),
+    lambda: q8.rmsnorm(meta(1, 2 ** 32 + 8, dtype=torch.float16), meta(2 ** 32 + 8, dtype=torch.float32)),
+    lambda: q8.dequantize(meta(1, 2 ** 32 + 8), meta(1, dtype=torch.float32)),
+    lambda: q8.gemm(meta(1, 2 ** 32 + 8), meta(1, dtype=torch.float32), meta(1, 2 ** 32 + 8), meta(1, dtype=torch.float32)),
+    lambda: q8._batch(q8.Batch(*(torch.zeros(n, dtype=torch.int32) for n in (1, 2, 1)), 1, 1), 2 ** 32 + 1, 0),
+])
+def test_sizes_past_32_bits_are_refused(call):
+    """ctypes would hand the library their low 32 bits: 8 columns, 1 row"""
+    with pytest.raises(ValueError, match=r"at most 2\^31 - 1"):
+        call()
+
+
+def test_products_wider_than_a_grid_are_refused(hip):
+    nobody = C.create_string_buffer(1 << 16)                 # a context of zeros: nothing of it is read before the checks
+    one = C.c_void_p(64)
+    assert hip.wj_q8_gemm(nobody, one, 16, one, one, 16, one, None, 0, one, 1 << 28, 1, 1 << 27, 16, None, 0, None) == -1
+    assert b"2^27 - 16" in hip.wj_last_error()

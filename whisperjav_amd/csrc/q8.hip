@@ -885,6 +885,7 @@ int wj_q8_gemm(wj_ctx* ctx, const int8_t* a_dev, int64_t lda, const float* a_sca
   WJ_REQUIRE(known_dtype(dtype), "wj_q8_gemm: unknown dtype %d", dtype);
   WJ_REQUIRE(m >= 0 && m <= (int64_t)65535 * 64 && n >= 0 && k >= 0 && k <= 131071, "wj_q8_gemm: %lld x %d x %d (at most 4194240 rows; k at most 131071: the sum is 32 bits wide)",
              (long long)m, n, k);
+  WJ_REQUIRE(n <= (1 << 27) - 16, "wj_q8_gemm: %d columns (at most 2^27 - 16: a grid's axis holds 2^32 threads, 32 for each)", n);
   if (m == 0 || n == 0) return WJ_OK;
   WJ_REQUIRE(a_scale_dev && w_scale_dev && out_dev && (k == 0 || (a_dev && w_dev)), "wj_q8_gemm: NULL argument");
   WJ_REQUIRE(lda >= 0 && ldw >= 0 && (m == 1 || ldo >= n), "wj_q8_gemm: output rows overlap (stride below %d columns)", n);

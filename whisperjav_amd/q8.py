@@ -34,6 +34,7 @@ from . import hipbind
 from .hipbind import WJ_BF16, WJ_F16, WJ_F32
 
 _TYPE = {torch.float32: WJ_F32, torch.float16: WJ_F16, torch.bfloat16: WJ_BF16}
+_INT = 2 ** 31 - 1                       # sizes that the library takes as 32-bit integers
 _STREAM_DEFAULT = C.c_void_p(-1)        # include/wjhip.h: WJ_STREAM_DEFAULT
 
 
@@ -77,6 +78,8 @@ def _float_rows(t: torch.Tensor, what: str, index: Optional[int] = None, rows: i
     shape = t.shape
     if len(shape) != 2 or (index is not None and (shape[0] != rows or shape[1] != cols)):
         raise ValueError(f"{what}: {'[rows, cols]' if index is None else [rows, cols]} expected, got {list(shape)}")
+    if shape[1] > _INT:
+        raise ValueError(f"{what}: {shape[1]} columns (at most 2^31 - 1)")
     if not t.is_cuda or (index is not None and t.get_device() != index):
         raise ValueError(f"{what}: on {t.device}, expected {'a GPU' if index is None else f'cuda:{index}'}")
     if t.stride(1) != 1 and shape[1] > 1:
@@ -89,6 +92,8 @@ def _codes(t: torch.Tensor, scale: torch.Tensor, what: str, index: Optional[int]
     """Check int8 rows and their scales; the GPU's index."""
     if t.dtype != torch.int8 or t.dim() != 2:
         raise ValueError(f"{what}: int8 [rows, cols] expected, got {t.dtype} {list(t.shape)}")
+    if t.shape[1] > _INT:
+        raise ValueError(f"{what}: {t.shape[1]} columns (at most 2^31 - 1)")
     if not t.is_cuda or (index is not None and t.get_device() != index):
         raise ValueError(f"{what}: on {t.device}, expected {'a GPU' if index is None else f'cuda:{index}'}")
     if t.stride(1) != 1 and t.shape[1] > 1:
@@ -192,6 +197,8 @@ def gemm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch
     (m, k), n = a.shape, w.shape[0]
     if w.shape[1] != k:
         raise ValueError(f"a has {k} columns, w has {w.shape[1]}")
+    if n > _INT:
+        raise ValueError(f"w: {n} rows (at most 2^31 - 1)")
     if bias is not None:
         _vector(bias, "bias", n, index)
     given = out
@@ -274,6 +281,8 @@ def _cache(cache: KV8Cache) -> Kv8C:
         raise ValueError("cache: int8 codes and float32 scales expected")
     if not (k.is_cuda and k.device == v.device == ks.device == vs.device):
         raise ValueError("cache: the four tensors must be on one GPU")
+    if max(shape) > _INT:
+        raise ValueError(f"cache: {list(shape)} (sizes of at most 2^31 - 1)")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache: contiguous tensors expected")
     c = Kv8C(*at[:4], *shape)
@@ -287,11 +296,13 @@ def _batch(batch: Batch, rows: int, index: int) -> Kv8BatchC:
     known = batch.__dict__.get("_c")
     if known is not None and known[0] == at:
         return known[1]
+    if rows > _INT:
+        raise ValueError(f"{rows} rows (at most 2^31 - 1)")
     n = slots.shape[0] if slots.dim() == 1 else -1
     for t, what, want in ((slots, "slots", n), (starts, "starts", n + 1), (lens, "lens", n)):
         if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != want or t.get_device() != index or not t.is_contiguous():
             raise ValueError(f"batch.{what}: contiguous int32 [{want if want >= 0 else 'seqs'}] on cuda:{index} expected, got {t.dtype} {list(t.shape)} on {t.device}")
-    b = Kv8BatchC(*at[:3], n, rows, max_new, max_len)
+    b = Kv8BatchC(*at[:3], n, rows, min(max_new, _INT), min(max_len, _INT))
     batch.__dict__["_c"] = (at, b)
     return b
 
