@@ -1,27 +1,17 @@
 """The arithmetic of the attention over the 8-bit cache (whisperjav_amd/q8.py): what its precision is, not only that it is right.
 
-Every kernel that a call can take is reached: PLANS names them by what sends a call there."""
-import math
-
+Every kernel that a call can take is reached, with both head dimensions."""
 import pytest
 import torch
 
 from tests import q8_ref as ref
+from tests.q8_cases import ATTENTION
 
 pytestmark = pytest.mark.gpu
 
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 
-# sequences, new rows, positions, heads, queries per head, dim
-PLANS = {
-    "four_waves": (3, 1, 120, 2, 2, 128),                # 16 rows, up to 128 positions
-    "eight_waves": (3, 2, 700, 2, 2, 128),               # 16 rows, more of them
-    "parts": (2, 1, 2500, 1, 4, 128),                    # positions split over workgroups and joined
-    "two_blocks": (2, 20, 300, 2, 1, 128),               # 32 rows
-    "two_blocks_parts": (2, 20, 1300, 1, 1, 128),
-    "many_rows": (26, 70, 110, 10, 1, 128),              # 128 rows (float32: 32)
-}
-CASES = [(name, *plan[:5], dim) for name, plan in PLANS.items() for dim in (64, 128)]
+CASES = [(name, *sizes, dim) for name, (sizes, _) in ATTENTION.items() for dim in (64, 128)]
 IDS = [f"{c[0]}-{c[6]}" for c in CASES]
 
 

@@ -18,7 +18,7 @@ CSRC = Path(__file__).resolve().parent / "csrc"
 LIB = CSRC / "libwjhip.so"
 SOURCES = ["engine.hip", "gemm.hip", "attention.hip", "norm.hip", "sampler.hip", "logmel.hip", "vad.hip", "vadgraph.hip", "align.hip", "comm.hip", "qwen.hip", "qwen_audio.hip", "q8.hip", "kv8.hip"]
 HEADERS = ["common.hpp", "attr_once.hpp", "kernels.hpp", "../../include/wjhip.h"]
-OWN_HEADERS = {"q8.hip": ["q8.hpp"], "kv8.hip": ["q8.hpp", "q8_plan.hpp"]}        # headers that only these sources include
+OWN_HEADERS = {"q8.hip": ["q8.hpp", "q8_plan.hpp"], "kv8.hip": ["q8.hpp", "q8_plan.hpp"]}        # headers that only these sources include
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Wno-unused-result"]
 # packed float32 instructions, which hipcc makes out of ordinary float code by itself: some of their forms have given wrong results on
 # MI355X now and then, with no error.  Off for the 8-bit operators.  The older sources keep them: without them the last bits of the word

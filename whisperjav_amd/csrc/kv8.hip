@@ -684,7 +684,10 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(const AttnArgs a, in
 }
 
 // the launch's sizes go by the hints as far as they can be true
-int most_new(const wj_kv8_batch& b) { return b.max_new < 1 ? 1 : b.max_new < b.rows ? b.max_new : b.rows; }
+int most_new(const wj_kv8_batch& b) { return wj::most_new(b.max_new, b.rows); }
+AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
+  return wj::plan_attention(c.heads, c.ctx, c.dim, b.seqs, most_new(b), b.max_len, n_heads);
+}
 
 int check_kv8(const char* who, wj_ctx* ctx, const wj_kv8* c, const wj_kv8_batch* b, int dtype) {
   WJ_REQUIRE(ctx && c && b, "%s: NULL argument", who);
@@ -738,38 +741,6 @@ int launch_read(const wj_kv8* c, const wj_kv8_batch* b, int dtype, void* k, int6
   if (dtype == WJ_F32) return start_read<float, 64>(c, b, k, ldk, v, ldv, pairs, s);
   if (dtype == WJ_F16) return start_read<f16_t, 64>(c, b, k, ldk, v, ldv, pairs, s);
   return start_read<bf16_t, 64>(c, b, k, ldk, v, ldv, pairs, s);
-}
-
-// Rows and waves per workgroup and parts per row, from the call's sizes alone (the workspace follows from them).  Measured on the MI355X (us a
-// call in a graph; float16, 8 heads of 128 and 1 .. 4 queries each unless said otherwise):
-//   16 rows, up to 1024 positions, four / eight waves: 16 sequences x 500 9.1 / 8.2, 16 x 1000 13.5 / 11.9, 64 x 500 13.2 / 15.8, 200 x 500
-//     36 / 49: eight where there are fewer than 256 workgroups (four parts and a join: 9.8 and 12.5, and 3.5 us more for the host);
-//   16 rows, more positions, one / two / four / eight parts: 1 x 4000 33 / 22 / 16 / 13, 16 x 4000 40 / 28 / 27 / 30, 64 x 1500 33 / 36 / 37 / 39,
-//     16 x 20 heads of 64 x 4000 45 / 37 / 34 / 37;
-//   32 rows: 1 x 1000 16 / 14 / 12 / 12, 16 x 1000 18 / 17 / 19 / 25, 16 x 4000 53 / 35 / 34 / 40, 64 x 1000 29 / 39 / 49 / 72, 1 x 500 10.6 / 11 / 10.3.
-// So parts make up to 512 workgroups, of 256 positions or more, at most 8.
-// The 128-row kernel against 32 rows per workgroup, new rows x queries per head, positions: 16 x 100 x 1, 500 25.7 / 19.0; 8 x 128 x 2, 1500 63.5 / 40;
-//   32 x 33 x 2, 500 26.1 / 26.0; 32 x 100 x 1, 500 and 1500 28.0 / 32.3 and 66 / 69; 4 x 500 x 2, 500 24.5 / 29.5; 16 x 500 x 2, 500 45 / 101;
-//   of 64 dims 32 x 100 x 1, 500 and 1500 20.9 / 21.8 and 53 / 47: a CU holds two of its workgroups, so it is for calls of more than three blocks
-//   of 32 rows per CU; up to 64 rows a sequence its waves would stand half idle (16 x 64 rows 24.0 / 12.6, 32 x 64 25.2 / 19.1).
-struct AttnPlan { int rt, waves, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel (16-bit types; float32 rows take two blocks)
-constexpr int kWhole = 0x40000000;
-AttnPlan plan_attention(const wj_kv8& c, const wj_kv8_batch& b, int n_heads) {
-  const int per = n_heads / c.heads;
-  const int64_t rows = (int64_t)most_new(b) * per;
-  const int64_t tiles = (int64_t)b.seqs * c.heads * ((rows + 127) / 128);
-  const int64_t blocks32 = (int64_t)b.seqs * c.heads * ((rows + 31) / 32);
-  if (rows > 64 && blocks32 > 768 && tiles < 1 << 22 && (int64_t)c.ctx * c.dim < 0x7fff0000) return {0, 4, 1, kWhole};
-  const int rt = rows <= 16 ? 1 : 2;
-  const int64_t groups = (int64_t)b.seqs * c.heads * ((rows + 16 * rt - 1) / (16 * rt));
-  const int len = b.max_len < c.ctx ? (b.max_len > 0 ? b.max_len : 1) : c.ctx;
-  if (rt == 1 && len <= 1024) return {1, len > 128 && groups < 256 ? 8 : 4, 1, kWhole};
-  int64_t parts = (512 + groups - 1) / groups;
-  parts = parts > 8 ? 8 : parts;
-  parts = parts > (len + 255) / 256 ? (len + 255) / 256 : parts;
-  if (parts <= 1 || (rt == 2 && len <= 512)) return {rt, 4, 1, kWhole};
-  const int chunk = (int)(((len + parts - 1) / parts + 127) / 128 * 128);
-  return {rt, 4, (len + chunk - 1) / chunk, chunk};
 }
 
 template <typename T, int HD, int RT>

@@ -3,6 +3,7 @@
 #include <type_traits>
 
 #include "q8.hpp"
+#include "q8_plan.hpp"
 
 using namespace wj;
 
@@ -739,31 +740,6 @@ int launch_rows(wj_ctx* ctx, int dtype, int delta_dtype, const RowArgs& a, void*
   if (dtype == WJ_F32) return pick_delta<MODE, float>(a, delta_dtype, s);
   if (dtype == WJ_F16) return pick_delta<MODE, f16_t>(a, delta_dtype, s);
   return pick_delta<MODE, bf16_t>(a, delta_dtype, s);
-}
-
-// Which kernel a product takes, from its size alone (the workspace follows from it).  Measured on the MI355X, us per call in a graph:
-//   rows / tile: 16 x 5176 x 5824 10.3 / 11.5, 48 x 4096 x 2048 6.3 / 8.6, 64 x 4096 x 2048 7.1 / 9.4, 64 x 12288 x 2048 17.0 / 10.3,
-//     32 x 5176 x 5824 14.2 / 11.8: the rows kernel reads the activations once per 16 columns, so beyond 16 rows it is for products where
-//     that is at most 36 MiB;
-//   tile / big: 2048 x 4096 x 2048 27.6 / 29.6, 3000 x 2048 x 6144 53 / 67, 512 x 12288 x 2048 22 / 30, 1024 x 12288 x 2048 40 / 32,
-//     3000 x 4096 x 2048 39 / 31, 1500 x 12288 x 2048 58 / 58: a round of 256 big tiles, filled or not, takes as long as 1000 small ones;
-//   tile of 64 / 128 rows: 512 x 5176 x 5824 39 / 31, 3000 x 1190 x 3808 31 / 25, 240 x 12288 x 2048 15.6 / 15.2, 384 x 5176 x 5824 24 / 31, 512 x
-//     12288 x 2048 22.6 / 26.9: the larger pays where small ones would share CUs unevenly and large ones have a CU each;
-//   big, stores past the caches: 16384 x 12288 x 2048 (402 MB out) 440 -> 398, 8192 x 12288 x 2048 (201 MB) 188 -> 208: for outputs beyond the
-//     256 MiB of the memory-side cache;
-//   tile, slices 1 / 2 / 4: 100 x 4096 x 2048 10.0 / 11.1 / 11.6, 100 x 2048 x 6144 23 / 15 / 12.5, 512 x 2048 x 6144 22.5 / 19.1 / 19.8: a
-//     slice saves its share of the 0.4 us that a step takes and the join costs 3 us, so it pays from 16 steps a slice while CUs are idle.
-enum GemmKind { GEMM_ROWS, GEMM_BIG, GEMM_TILE, GEMM_TILE128 };
-struct GemmPlan { GemmKind kind; int ksplit; };
-GemmPlan plan_gemm(int64_t m, int n, int k) {
-  if (m <= 16 || (m <= 64 && m * k * ((n + 15) / 16) <= (int64_t)36 << 20)) return {GEMM_ROWS, 1};
-  const int64_t t256 = ((m + 255) / 256) * ((n + 255) / 256), t64 = ((m + 63) / 64) * ((n + 127) / 128);
-  if (t64 > 1000 * ((t256 + 255) / 256)) return {GEMM_BIG, 1};
-  if (t64 > 256 && ((m + 127) / 128) * ((n + 127) / 128) <= 256) return {GEMM_TILE128, 1};
-  const int steps = (k + 127) / 128;
-  int ks = 1;
-  while (ks < 8 && t64 * ks * 2 <= 256 && steps > 16 * ks) ks *= 2;
-  return {GEMM_TILE, ks};
 }
 
 template <typename K>
