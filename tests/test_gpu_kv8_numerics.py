@@ -138,3 +138,12 @@ def test_largest_rows_written_and_read_by_attention(q8, dtype, positions):
     got = q8.kv_attention(torch.ones(positions, 2, 64).to(dtype).cuda(), cache, batch).cpu().double()
     held = cache.v[0, :, 0].cpu().double() * cache.v_scale[0, :, 0].cpu().double()[:, None]
     assert bool(((got - held).abs() <= (2.0 ** -17 + {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}[dtype]) * held.abs()).all())
+
+
+@pytest.mark.parametrize("case", CASES, ids=IDS)
+def test_float32_outputs_are_good_to_18_bits(q8, case):
+    """Weights are off by 2^-18 at most (see the value scales' test), each for itself: so is the sum of weight x value against its own norm.  Queries of
+    one half would make it 2^-12 / sqrt(3) of a score of about 1.7 (in units of log2), 1.7e-4; numerators of one half 2^-12 / sqrt(3), 1.4e-4."""
+    q, host, starts, lens = make(q8, rng(case[3] + case[6]), case, torch.float32)
+    got, want, _ = attend(q8, q, host, starts, lens)
+    assert float((got.double() - want).norm() / want.norm()) <= 2.0 ** -18
