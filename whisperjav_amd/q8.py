@@ -232,7 +232,7 @@ class _CacheTensors(NamedTuple):
 
 class KV8Cache(_CacheTensors):
     """One layer's keys and values in 8 bits: codes int8 ``[slots, heads, ctx, dim]`` and scales float32 ``[slots, heads, ctx]``.
-    A program keeps it like a handle: the tensors are checked at its first use, and again when one of them has other memory or another size."""
+    A program keeps it like a handle: the tensors are checked at its first use, and again when one of them has other memory."""
 
     @classmethod
     def empty(cls, slots: int, heads: int, ctx: int, dim: int, device: torch.device = torch.device("cuda", 0)) -> "KV8Cache":
@@ -265,12 +265,17 @@ class Batch(_BatchArrays):
         return type(self), tuple(self)
 
 
+def _storages(tensors) -> list:
+    """Kept beside addresses: while memory is held, no other tensor can come to lie at its address."""
+    return [t.untyped_storage() for t in tensors]
+
+
 def _cache(cache: KV8Cache) -> Kv8C:
     k, ks, v, vs = cache
     _no_gradient(ks, "cache scale")
     _no_gradient(vs, "cache scale")
-    at = (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), k.numel(), ks.numel(), v.numel(), vs.numel())
-    known = cache.__dict__.get("_c")             # checked and laid out at the object's first use
+    at = (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr())
+    known = cache.__dict__.get("_c")             # checked and laid out at the object's first use; see _storages
     if known is not None and known[0] == at:
         return known[1]
     shape = k.shape
@@ -285,14 +290,14 @@ def _cache(cache: KV8Cache) -> Kv8C:
         raise ValueError(f"cache: {list(shape)} (sizes of at most 2^31 - 1)")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("cache: contiguous tensors expected")
-    c = Kv8C(*at[:4], *shape)
-    cache.__dict__["_c"] = (at, c)
+    c = Kv8C(*at, *shape)
+    cache.__dict__["_c"] = (at, c, _storages(cache))
     return c
 
 
 def _batch(batch: Batch, rows: int, index: int) -> Kv8BatchC:
     slots, starts, lens, max_new, max_len = batch
-    at = (slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), rows, index, slots.numel(), starts.numel(), lens.numel())
+    at = (slots.data_ptr(), starts.data_ptr(), lens.data_ptr(), rows, index)
     known = batch.__dict__.get("_c")
     if known is not None and known[0] == at:
         return known[1]
@@ -303,7 +308,7 @@ def _batch(batch: Batch, rows: int, index: int) -> Kv8BatchC:
         if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != want or t.get_device() != index or not t.is_contiguous():
             raise ValueError(f"batch.{what}: contiguous int32 [{want if want >= 0 else 'seqs'}] on cuda:{index} expected, got {t.dtype} {list(t.shape)} on {t.device}")
     b = Kv8BatchC(*at[:3], n, rows, min(max_new, _INT), min(max_len, _INT))
-    batch.__dict__["_c"] = (at, b)
+    batch.__dict__["_c"] = (at, b, _storages(batch[:3]))
     return b
 
 
