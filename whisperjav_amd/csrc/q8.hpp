@@ -1,4 +1,4 @@
-// q8.hpp -- what the 8-bit operators (q8.hip, kv8.hip) share: element access by run-time type, row quantisation, host-side checks.
+// q8.hpp -- what the 8-bit operators (q8.hip, kv8.hip) share: element types, row quantisation, host-side checks.
 #pragma once
 
 #include <math.h>
@@ -22,13 +22,6 @@ struct DeviceScope {
 inline bool known_dtype(int dtype) { return dtype == WJ_F32 || is16(dtype); }
 inline bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
-// one element of a row whose type is known at run time only (wave-uniform)
-__device__ __forceinline__ float ld_any(const void* p, int dtype, int64_t i) {
-  if (dtype == WJ_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == WJ_F16) return h2f(reinterpret_cast<const f16_t*>(p)[i]);
-  return bf2f(reinterpret_cast<const bf16_t*>(p)[i]);
-}
-
 // bfloat16 of any float, NaN included (f2bf's carry can turn a NaN's payload into an infinity): one instruction on gfx950
 __device__ __forceinline__ bf16_t f2bf_any(float v) { return __builtin_bit_cast(bf16_t, static_cast<__bf16>(v)); }
 template <typename T> __device__ __forceinline__ T to_T(float v);
@@ -36,6 +29,7 @@ template <> __device__ __forceinline__ float to_T<float>(float v) { return v; }
 template <> __device__ __forceinline__ f16_t to_T<f16_t>(float v) { return f2h(v); }
 template <> __device__ __forceinline__ bf16_t to_T<bf16_t>(float v) { return f2bf_any(v); }
 
+// one element of a row whose type is known at run time only (wave-uniform)
 __device__ __forceinline__ void st_any(void* p, int dtype, int64_t i, float v) {
   if (dtype == WJ_F32) reinterpret_cast<float*>(p)[i] = v;
   else if (dtype == WJ_F16) reinterpret_cast<f16_t*>(p)[i] = f2h(v);
