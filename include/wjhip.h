@@ -509,7 +509,8 @@ int wj_q8_quantize(wj_ctx* ctx, int dtype, const void* x_dev, int64_t ldx, int s
 int wj_q8_dequantize(wj_ctx* ctx, const int8_t* codes_dev, int64_t ldc, const float* scale_dev, int dtype, void* out_dev, int64_t ldo,
                      int64_t rows, int cols, void* stream);
 /* out [m][n] in `dtype` = a_scale[i] * w_scale[j] * sum_k a[i][k] w[j][k] + bias[j] (bias float32 [n] or NULL).  The sum is exact
- * (int32; codes may be -128 too, hence k <= 131071); the epilogue is float32, rounded once.  lda, ldw >= k.  Rows of codes that start at
+ * (int32; codes may be -128 too, hence k <= 131071); the epilogue is float32, rounded once, the product of the two scales first (it has to
+ * lie inside float32's normal range).  lda, ldw >= k.  Rows of codes that start at
  * multiples of 16 bytes take the fast kernels (bytes between k and the next multiple of 16 are read and ignored, never written); any
  * other base or stride is served, slower.  workspace_dev: at least wj_q8_gemm_workspace() bytes (may be 0 and NULL), used by this call
  * alone until it is done on `stream`.  At most 4194240 rows and 2^27 - 16 columns. */
@@ -533,7 +534,8 @@ typedef struct {
  * rows behind starts[seqs] are neither read nor written.  A sequence whose slot is outside 0 .. slots - 1 (a padded batch entry: -1)
  * stores nothing, reads back as zeros and attends to nothing; so does, in writing and reading, a row whose position is outside
  * 0 .. ctx - 1.  max_new, max_len: the most new rows and positions of any sequence -- hints that size the launch: a call whose arrays go
- * past them is still right, only slower. */
+ * past them is still right, only slower.  They choose the attention's kernel, so its results under other hints may differ in their last
+ * bits.  Entries that are no spans (a start before row 0 or behind the next one) own no rows, a negative length is none. */
 typedef struct {
   const int32_t* slots_dev;
   const int32_t* starts_dev;
@@ -551,7 +553,9 @@ int wj_kv8_read(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int
  * (causal != 0) or j < lens[b] (causal = 0: an encoder's states of another length, written once), the first ctx positions at most.
  * q, out [rows][n_heads][dim] in `dtype`; query head h reads key / value head h / (n_heads / heads), n_heads <= 16 heads.  A row that
  * sees no position (an empty cache, a causal row before position 0) is zeros.
- * Positions behind are never let into a result, whatever the cache holds there.  Scores, softmax and sums are float32.
+ * Positions behind are never let into a result, whatever the cache holds there.  Scores, softmax and sums are float32; a float32 or
+ * bfloat16 query enters as two halves or one in units of its row's largest value (22 bits, 2^-25 of that value at least), a softmax weight
+ * times its value's scale as two (21 bits).  Values may be of any finite size; below 1e-29 they lose bits.
  * workspace_dev: at least wj_kv8_attention_workspace() bytes (may be 0 and NULL), used by this call alone until it is done on `stream`. */
 int64_t wj_kv8_attention_workspace(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int n_heads);
 int wj_kv8_attention(wj_ctx* ctx, const wj_kv8* cache, const wj_kv8_batch* batch, int dtype, const void* q_dev, int64_t ldq, void* out_dev,

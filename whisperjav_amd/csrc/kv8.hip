@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, T* __res
 // M moves only when the largest numerator would pass 2^15.  The smallest step of a half, 2^-24, is then 2^-34 of the row's largest numerator or
 // less: what a weight can lose for being small.  A numerator goes into the product as a high and a low half (21 bits or more): the results are
 // those of the float32 form.  With one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 and a bfloat16 row 1.671e-3 instead of 1.658e-3 (8 % of its values are not the nearest ones, against 0.06 %); the second product costs nothing where
-// memory bounds the call (512 sequences 124 us) and 10 % of a bfloat16 prompt pass (32 prompts 142 -> 157 us).
+// memory bounds the call (512 sequences 124 us) and 11 to 16 % of a bfloat16 prompt pass (32 prompts 142 -> 157 us).
 // --------------------------------------------------------------------------------------------
 struct AttnArgs {
   Kv8Args s;
@@ -458,8 +458,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(void* p, int bytes) 
 // halves ONCE per workgroup on their way into LDS (both operands in the order the products read them: K rows permuted, V transposed in
 // registers, 8 positions of one dimension per 16-byte piece), which the rows kernel above does once per wave.  The next 64 positions are
 // in flight (registers) while this wave's products run.  Two buffers, one barrier per step, two workgroups per CU.  Bound by the vector unit
-// (widening, softmax) beside the matrix pipe: 32 bfloat16 prompts of 250 .. 1000 positions, 16 heads on 8 of 128, 142 us (299 with 32 rows per
-// workgroup); 4 of 4000 positions, 32 heads on 8, 690 us, 760 TFLOP/s of what the causal mask leaves.
+// (widening, softmax; busy 50 % of the cycles) beside the matrix pipe (24 %): 32 bfloat16 prompts of 250 .. 1000 positions, 16 heads on 8 of 128, 157 us
+// (299 with 32 rows per workgroup, when a numerator was one half); 4 of 4000 positions, 32 heads on 8, 823 us, 637 TFLOP/s of what the causal mask
+// leaves; float16 148 and 791 us.
 template <typename T, int HD>
 __global__ __launch_bounds__(256, 2) void kv8_attn_tile_kernel(const AttnArgs a, int blocks) {
   constexpr int NP = 1;

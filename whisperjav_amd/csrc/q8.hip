@@ -372,7 +372,7 @@ __device__ __forceinline__ void tile_of(int lin, int nx, int ny, int* tx, int* t
 // WAR: the other buffer held pair p - 1, read last in group 1's MEM(2p - 1), retired before B(4p - 1); MEM(2p) starts after it.
 // RAW: both groups have waited for pair p + 1 by B(4p + 3); it is first read after that.
 // 128-byte LDS rows, 16-byte piece c of row r in place c ^ (r & 7).
-// Bound by the matrix pipe: 16384 x 12288 x 2048 in 395 us, 2.09 POP/s.
+// 16384 x 12288 x 2048 in 387 .. 402 us, 2.05 .. 2.13 POP/s: the matrix pipe is busy half of the cycles, at a clock that falls to 2 GHz under it.
 template <typename T, bool PAST>
 __global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, int nx, int ny) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [buffer][A | W][256][128]
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(512) void q8_gemm_big_kernel(const GemmQ8Args g, in
 // each four taking one half of every step's codes, so that the two waves of a SIMD overlap one's LDS reads with the other's products; the
 // two halves' sums meet in LDS at the end, each four finishing half of the rows.  For calls with too few 256-tiles to fill the chip;
 // ksplit > 1: slices of k on the grid's second axis write raw sums, joined by q8_gemm_join_kernel.  Bound by LDS traffic (DMA in, fragments out):
-// 240 x 12288 x 2048 in 14 us, 0.38 us per step of a 64-row tile (0.23 with the DMA taken away).
+// 0.38 us per step of a 64-row tile (300 x 2048 x 8192; 0.23 with the DMA taken away); 240 x 12288 x 2048 takes 128-row tiles, 14 us.
 template <typename T, int BM>
 __global__ __launch_bounds__(512) void q8_gemm_tile_kernel(const GemmQ8Args g, int nx, int ny) {
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];      // [stage][A: BM | W: 128][128]

@@ -17,7 +17,8 @@ constexpr Span span_from(int slot, int first, int last, int len, int slots, int 
   return Span{slot >= 0 && slot < slots ? slot : -1, there ? first : rows, n, positions, positions - n};
 }
 
-// Which kernel a product takes, from its size alone (the workspace follows from it).  Measured on the MI355X, us per call in a graph:
+// Which kernel a product takes, from its size alone (the workspace follows from it).  Measured on the MI355X, us per call in a graph (both sides of a pair
+// in one run; runs differ by up to 10 %):
 //   rows / tile: 16 x 5176 x 5824 10.3 / 11.5, 48 x 4096 x 2048 6.3 / 8.6, 64 x 4096 x 2048 7.1 / 9.4, 64 x 12288 x 2048 17.0 / 10.3,
 //     32 x 5176 x 5824 14.2 / 11.8: the rows kernel reads the activations once per 16 columns, so beyond 16 rows it is for products where
 //     that is at most 36 MiB;
@@ -50,12 +51,12 @@ constexpr int most_new(int max_new, int rows) { return max_new < 1 ? 1 : max_new
 //   16 rows, up to 1024 positions, four / eight waves: 16 sequences x 500 9.1 / 8.2, 16 x 1000 13.5 / 11.9, 64 x 500 13.2 / 15.8, 200 x 500
 //     36 / 49: eight where there are fewer than 256 workgroups (four parts and a join: 9.8 and 12.5, and 3.5 us more for the host);
 //   16 rows, more positions, one / two / four / eight parts: 1 x 4000 33 / 22 / 16 / 13, 16 x 4000 40 / 28 / 27 / 30, 64 x 1500 33 / 36 / 37 / 39,
-//     16 x 20 heads of 64 x 4000 45 / 37 / 34 / 37;
+//     16 x 20 heads of 64 x 4000 45 / 37 / 34 / 37 (more parts were not measured);
 //   32 rows: 1 x 1000 16 / 14 / 12 / 12, 16 x 1000 18 / 17 / 19 / 25, 16 x 4000 53 / 35 / 34 / 40, 64 x 1000 29 / 39 / 49 / 72, 1 x 500 10.6 / 11 / 10.3.
 // So parts make up to 512 workgroups, of 256 positions or more, at most 8.
 // The 128-row kernel against 32 rows per workgroup, new rows x queries per head, positions: 16 x 100 x 1, 500 25.7 / 19.0; 8 x 128 x 2, 1500 63.5 / 40;
 //   32 x 33 x 2, 500 26.1 / 26.0; 32 x 100 x 1, 500 and 1500 28.0 / 32.3 and 66 / 69; 4 x 500 x 2, 500 24.5 / 29.5; 16 x 500 x 2, 500 45 / 101;
-//   of 64 dims 32 x 100 x 1, 500 and 1500 20.9 / 21.8 and 53 / 47: a CU holds two of its workgroups, so it is for calls of more than three blocks
+//   of 64 dims 32 x 100 x 1, 500 and 1500 20.9 / 21.8 and 53 / 47 (one border for both dims: this last one is on its wrong side): a CU holds two of its workgroups, so it is for calls of more than three blocks
 //   of 32 rows per CU; up to 64 rows a sequence its waves would stand half idle (16 x 64 rows 24.0 / 12.6, 32 x 64 25.2 / 19.1).
 struct AttnPlan { int rt, waves, nsplit, chunk; };        // rt: 16-row blocks per workgroup, 0: the 128-row kernel (16-bit types; float32 rows take two blocks)
 constexpr int kWhole = 0x40000000;

@@ -258,7 +258,8 @@ class _BatchArrays(NamedTuple):
 class Batch(_BatchArrays):
     """The sequences of a call, int32 on the device: sequence b owns rows ``starts[b] .. starts[b + 1] - 1`` of the row tensors and has
     ``lens[b]`` positions in slot ``slots[b]`` of the cache once they are written, the rows being the last ones.  A slot of -1 is padding.
-    ``max_new`` / ``max_len``: the most new rows / positions of any sequence; they size the launch (results do not depend on them).  The
+    ``max_new`` / ``max_len``: the most new rows / positions of any sequence; they size the launch.  A call is right whatever they say, but they choose
+    the kernel and with it the order of the sums: attention under other hints may differ in its last bits.  The
     arrays may change between replays of a captured graph.  Slots are distinct where the batch is written."""
 
     def __reduce__(self):

@@ -397,7 +397,7 @@ class HipWhisperModel:
             raise ValueError(f"HipWhisperModel runs on the MI355X only (device={device!r}); there is no CPU path")
         # ctranslate2 compute types -> engine arithmetic.  "float16" is the reference's own GPU arithmetic
         # (faster-whisper float16 / whisper fp16=True) and what "auto" resolves to on a GPU there
-        # (whisperjav/config/resolver_v3.py:163-168); the int8 flavours have no MI355X counterpart here and run
+        # (whisperjav/config/resolver_v3.py:163-168); this engine has no int8 weights: the int8 flavours run
         # in the 16-bit type they dequantise to.
         ct = {"auto": "float16", "default": "float16", "bfloat16": "bfloat16", "float16": "float16",
               "float32": "float32", "int8": "float16", "int8_float16": "float16", "int8_bfloat16": "bfloat16"}
