@@ -147,3 +147,23 @@ def test_float32_outputs_are_good_to_18_bits(q8, case):
     q, host, starts, lens = make(q8, rng(case[3] + case[6]), case, torch.float32)
     got, want, _ = attend(q8, q, host, starts, lens)
     assert float((got.double() - want).norm() / want.norm()) <= 2.0 ** -18
+
+
+@pytest.mark.parametrize("case", CASES, ids=IDS)
+@pytest.mark.parametrize("dtype,power", [(torch.float16, -18), (torch.float16, 9), (torch.bfloat16, -100), (torch.bfloat16, 100), (torch.float32, -100), (torch.float32, 100)])
+def test_queries_of_any_size(q8, case, dtype, power):
+    """queries 2^power times as large under a scale 2^-power times as large (float16 ones below 2^-14 have fewer bits: those they have count)"""
+    q, host, starts, lens = make(q8, rng(case[3] + case[6]), case, torch.float32)
+    q = (q.double() * 2.0 ** power).to(dtype)
+    seqs, scale = len(lens), q.shape[2] ** -0.5 * 2.0 ** -power
+    slots = list(range(seqs))
+    cache = q8.KV8Cache(*(t.cuda() for t in host))
+    batch = q8.Batch(ints(slots), ints(starts), ints(lens), max(b - a for a, b in zip(starts, starts[1:])), max(lens))
+    got = q8.kv_attention(q.cuda(), cache, batch, scale=scale).cpu()
+    k, v = (host[i].double() * host[i + 1].double()[..., None] for i in (0, 2))
+    want = ref.attention(q, k, v, slots, starts, lens, True, scale)
+    if dtype == torch.float32:
+        assert float((got.double() - want).norm() / want.norm()) <= 2.0 ** -18
+    else:
+        off = float((got != want.to(dtype)).double().mean())
+        assert off <= {torch.float16: 0.04, torch.bfloat16: 0.01}[dtype], off

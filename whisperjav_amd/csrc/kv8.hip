@@ -95,8 +95,9 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Args a, T* __res
 // Exponents below -90 count as -90, so that a term is at most 2^105: scales below 2^-105 lose bits of their numerators.
 // M moves only when the largest numerator would pass 2^15.  The smallest step of a half, 2^-24, is then 2^-34 of the row's largest numerator or
 // less: what a weight can lose for being small.  A numerator goes into the product as a high and a low half (21 bits or more): the results are
-// those of the float32 form.  With one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 and a bfloat16 row 1.671e-3 instead of 1.658e-3 (8 % of its values are not the nearest ones, against 0.06 %); the second product costs nothing where
-// memory bounds the call (512 sequences 124 us) and 11 to 16 % of a bfloat16 prompt pass (32 prompts 142 -> 157 us).
+// those of the float32 form.  With one half a float16 row ends up 3.0e-4 off instead of 2.1e-4 and a bfloat16 row 1.671e-3 instead of 1.658e-3
+// (8 % of its values are not the nearest ones, against 0.06 %); the second product costs nothing where memory bounds the call (512 sequences
+// 124 us) and 11 to 16 % of a bfloat16 prompt pass (32 prompts 142 -> 157 us).
 // --------------------------------------------------------------------------------------------
 struct AttnArgs {
   Kv8Args s;
